@@ -78,6 +78,13 @@ enum scn_precision {
                              NaN (its low part is inf - inf).  (The name is kept from the first form, three
                              tf32 products of a tf32 hi / lo split, which SCN_X3_FORM=tf32 still selects.) */
 };
+/* what the values of a matrix are, for the operators that take more than float32 */
+enum scn_type {
+  SCN_TYPE_FLOAT32 = 0,
+  SCN_TYPE_BFLOAT16 = 1,
+  SCN_TYPE_FLOAT16 = 2,
+  SCN_TYPE_E4M3 = 3 /* 8 bits: sign, 4 exponent bits, 3 of the mantissa, largest value 448, no infinities */
+};
 /* which convolution kernel the last convolution call of this thread ran (for profiling) */
 enum scn_conv_kernel {
   SCN_KERNEL_CONV_SIMT = 0,          /* k_conv_pipe / k_conv_simt / k_conv_thin: fp32 FMA     */
@@ -627,6 +634,25 @@ SCN_API int scn_unpooling_backward(scn_metadata *md, const int64_t *input_size, 
  * d_out_dense [batch, n_planes, *spatial_size] -> d_in [n_active, n_planes]. */
 SCN_API int scn_sparse_to_dense_backward(scn_metadata *md, const int64_t *spatial_size, float *d_in_features,
                                  const float *d_out_dense, int n_planes, void *stream);
+
+/* ---- Operators on rows of any kind --------------------------------------------------------------
+ * Rows of a matrix without a metadata object: the sites of a scale, points, tokens.  None of these is in the reference.
+ * Values are float32, bfloat16 or float16 (an scn_type); a row is contiguous, rows lie `stride` values apart where an
+ * argument says so and n_planes apart elsewhere.  Sums are float32; results are bit-reproducible. */
+
+/* Root-mean-square norm of every row of x, behind the addition of a residual (may be NULL):
+ *     s = x + residual, rounded to `type`      y = s / sqrt(mean(s s) + eps) * weight      (weight: NULL = ones)
+ * `sum` receives s (NULL without a residual), `out` y as out_type; inv_rms [n_rows] (may be NULL) 1 / sqrt(..) for the
+ * backward call.  out_type SCN_TYPE_E4M3: scale [n_rows] receives a / 448 with a = max(max |y|, 1e-30) over the row,
+ * `out` y * (448 / a); a row with a NaN has a NaN for a scale. */
+SCN_API int scn_rms_norm_forward(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, int type,
+                                 const float *weight, int64_t n_rows, int n_planes, double eps, void *sum, void *out,
+                                 int out_type, float *scale, float *inv_rms, void *stream);
+/* Its gradients: s is what the forward call normalised (x itself without a residual).  d_x (= the residual's gradient)
+ * includes d_sum (may be NULL), the gradient that reached s from elsewhere; d_weight (may be NULL) is overwritten. */
+SCN_API int scn_rms_norm_backward(const void *s, int64_t s_stride, int type, const float *weight, const float *inv_rms,
+                                  const void *d_out, int d_out_type, const void *d_sum, int64_t n_rows, int n_planes,
+                                  void *d_x, float *d_weight, void *stream);
 
 #ifdef __cplusplus
 }

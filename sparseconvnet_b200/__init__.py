@@ -41,6 +41,7 @@ def Metadata(dim):
 
 from .layers import (InputLayer, OutputLayer, BLInputLayer, BLOutputLayer, SubmanifoldConvolution, ValidConvolution, Convolution,  # noqa: E402
                      Deconvolution, BatchNormalization, BatchNormReLU, BatchNormLeakyReLU, MaxPooling, AveragePooling, UnPooling,
-                     SparseToDense, NetworkInNetwork, Identity)
+                     SparseToDense, NetworkInNetwork, RMSNormalization, AddRMSNormalization, Identity)
+from .rows import rms_norm, rms_norm_quantized  # noqa: E402
 from .containers import Sequential, ConcatTable, JoinTable, AddTable  # noqa: E402
 from .architectures import SparseVggNet, SparseResNet, UNet, FullyConvolutionalNet  # noqa: E402

@@ -68,6 +68,10 @@ SIGNATURES = {
                                             C.POINTER(C.c_double)]),
     "scn_batchnorm_join_forward": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_double,
                                              C.c_double, _vp]),
+    "scn_rms_norm_forward": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, C.c_int, _vp, C.c_int64, C.c_int, C.c_double, _vp, _vp,
+                                       C.c_int, _vp, _vp, _vp]),
+    "scn_rms_norm_backward": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, _vp, _vp,
+                                        _vp]),
     "scn_rows_affine_forward": (C.c_int, [_vp, _vp, C.c_int64, C.c_int, C.c_int, _vp, _vp, _vp]),
     "scn_rows_affine_backward": (C.c_int, [_vp, _vp, C.c_int64, C.c_int, C.c_int, _vp, _vp, _vp]),
     "scn_batchnorm_fold": (C.c_int, [_vp, _vp, _vp, _vp, C.c_double, C.c_int, _vp, _vp, _vp]),

@@ -17,8 +17,8 @@ def _flatten(seq, out):
 
 def _keeps_sites(m):
     """True for a module whose output has the sites and the spatial size of its input."""
-    if isinstance(m, (layers.SubmanifoldConvolution, layers.BatchNormalization, layers.Identity, layers.NetworkInNetwork,
-                      AddTable, JoinTable)):
+    if isinstance(m, (layers.SubmanifoldConvolution, layers.BatchNormalization, layers.RMSNormalization, layers.Identity,
+                      layers.NetworkInNetwork, AddTable, JoinTable)):
         return True
     if type(m) is Sequential:
         return all(_keeps_sites(c) for c in m._modules.values())

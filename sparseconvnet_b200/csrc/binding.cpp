@@ -1060,6 +1060,156 @@ SCN_FN(versions) {
   SCN_END
 }
 
+// ---- operators on rows of any kind (rows.py) ----------------------------------------------------------------------------
+int type_of(const at::Tensor &t, const char *name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return SCN_TYPE_FLOAT32;
+    case at::kBFloat16: return SCN_TYPE_BFLOAT16;
+    case at::kHalf: return SCN_TYPE_FLOAT16;
+    default: fail("%s must be float32, bfloat16 or float16", name);
+  }
+}
+
+const at::Tensor &on_gpu(PyObject *o, const char *name) {
+  const at::Tensor &t = tensor(o, name);
+  if (!t.is_cuda()) fail("%s must be a CUDA tensor: sparseconvnet_b200 has no CPU path", name);
+  return t;
+}
+
+// [.., planes] as a matrix whose rows are contiguous (a copy only where they are not)
+at::Tensor as_rows(const at::Tensor &t) {
+  const int64_t planes = t.size(-1);
+  if (t.dim() == 2 && (t.stride(1) == 1 || planes == 1) && t.stride(0) >= 0) return t;
+  const int64_t rows = planes ? t.numel() / planes : 0;
+  return t.contiguous().view({rows, planes});
+}
+void *raw(const at::Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+int64_t row_stride(const at::Tensor &t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : t.defined() ? t.size(1) : 0; }
+
+// float32 [planes] on the rows' device, or None
+at::Tensor row_weight(PyObject *o, const at::Tensor &like, int64_t planes) {
+  if (o == Py_None) return at::Tensor();
+  const at::Tensor &t = on_gpu(o, "weight");
+  if (t.scalar_type() != at::kFloat) fail("weight must be float32");
+  if (t.dim() != 1 || t.size(0) != planes) fail("weight must have %lld entries", (long long)planes);
+  if (t.device() != like.device()) fail("weight is on another device than the rows");
+  return t;
+}
+
+struct RmsNormNode : ag::Node {
+  ag::SavedVariable rows_, weight_;
+  at::Tensor inv_rms;
+  std::vector<int64_t> shape;
+  bool with_sum = false, with_weight = false;
+  std::string name() const override { return "RmsNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    rows_.reset_data();
+    weight_.reset_data();
+    inv_rms.reset();
+  }
+  ag::variable_list apply(ag::variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ag::variable_list result(3);
+    const bool from_out = grads[0].defined(), from_sum = with_sum && grads[1].defined();
+    if (!from_out && !from_sum) return result;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm: its gradient cannot be differentiated again (create_graph)");
+    const bool rows_wanted = task_should_compute_output(0) || (with_sum && task_should_compute_output(1));
+    if (!from_out) {
+      if (task_should_compute_output(0)) result[0] = grads[1];
+      if (task_should_compute_output(1)) result[1] = grads[1];
+      return result;
+    }
+    const at::NoGradGuard no_grad;
+    const at::Tensor s = as_rows(rows_.unpack(with_sum ? shared_from_this() : nullptr));
+    const at::Tensor w = with_weight ? weight_.unpack().contiguous() : at::Tensor();
+    const at::Tensor dy = grads[0].contiguous(), ds = from_sum ? grads[1].contiguous() : at::Tensor();
+    const OnDevice on(s);
+    const int64_t n = s.size(0), planes = s.size(1);
+    at::Tensor dx = at::empty({n, planes}, s.options()), dw;
+    if (with_weight && task_should_compute_output(2)) dw = at::empty({planes}, w.options());
+    auto code = [](const at::Tensor &t) {
+      TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf,
+                  "the gradient must be float32, bfloat16 or float16");
+      return t.scalar_type() == at::kFloat ? SCN_TYPE_FLOAT32 : t.scalar_type() == at::kHalf ? SCN_TYPE_FLOAT16 : SCN_TYPE_BFLOAT16;
+    };
+    check_free(scn_rms_norm_backward(raw(s), row_stride(s), code(s), w.defined() ? (const float *)raw(w) : nullptr, (const float *)raw(inv_rms),
+                                     raw(dy), code(dy), raw(ds), n, (int)planes, raw(dx), dw.defined() ? (float *)raw(dw) : nullptr,
+                                     on.stream));
+    if (rows_wanted) dx = dx.view(shape);
+    if (task_should_compute_output(0)) result[0] = dx;
+    if (with_sum && task_should_compute_output(1)) result[1] = dx;
+    result[2] = dw;
+    return result;
+  }
+};
+
+// (x [.., planes], weight or None, residual or None, eps, type of the result: an scn_type or -1 for x's)
+//   -> y, or (y, x + residual); type SCN_TYPE_E4M3: (q, scale) or (q, scale, x + residual)
+SCN_FN(rms_norm) {
+  SCN_BEGIN(5)
+  const at::Tensor &x = on_gpu(a[0], "x");
+  const int type = type_of(x, "x");
+  const double eps = PyFloat_AsDouble(a[3]);
+  int out_type = (int)PyLong_AsLong(a[4]);
+  if (PyErr_Occurred()) throw Fail{};
+  if (out_type < 0) out_type = type;
+  if (x.dim() < 1 || x.size(-1) < 1) fail("x must have at least one plane");
+  if (x.size(-1) > (1ll << 30)) fail("x has too many planes");
+  if (!(eps >= 0)) fail("eps must not be negative");
+  const int64_t planes = x.size(-1);
+  const at::Tensor weight = row_weight(a[1], x, planes);
+  at::Tensor residual;
+  if (a[2] != Py_None) {
+    residual = on_gpu(a[2], "residual");
+    if (residual.sizes() != x.sizes() || residual.scalar_type() != x.scalar_type() || residual.device() != x.device())
+      fail("residual must have the shape, the type and the device of x");
+  }
+  no_tangents(x, weight, residual);
+  const bool quantized = out_type == SCN_TYPE_E4M3;
+  const bool grad = ag::compute_requires_grad(x, residual, weight);
+  if (quantized && grad) fail("a result in 8 bits has no gradient: call it under torch.no_grad() or on detached tensors");
+  at::Tensor rows, sum, out, scale, inv_rms;
+  {
+    const at::NoGradGuard no_grad;
+    rows = as_rows(x);
+    const at::Tensor other = residual.defined() ? as_rows(residual) : residual, w = weight.defined() ? weight.contiguous() : weight;
+    const OnDevice on(x);
+    const int64_t n = rows.size(0);
+    const at::ScalarType types[] = {at::kFloat, at::kBFloat16, at::kHalf, at::kFloat8_e4m3fn};
+    out = at::empty(x.sizes(), x.options().dtype(types[out_type]));
+    if (residual.defined()) sum = at::empty(x.sizes(), x.options());
+    if (quantized) scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    if (grad) inv_rms = at::empty({n}, x.options().dtype(at::kFloat));
+    SCN_CALL(scn_rms_norm_forward(raw(rows), row_stride(rows), raw(other), row_stride(other), type,
+                                  w.defined() ? (const float *)raw(w) : nullptr, n, (int)planes, eps, raw(sum), raw(out), out_type,
+                                  (float *)raw(scale), (float *)raw(inv_rms), on.stream));
+  }
+  if (grad) {
+    std::shared_ptr<RmsNormNode> node(new RmsNormNode(), ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(x, residual, weight));
+    node->inv_rms = inv_rms, node->shape = x.sizes().vec();
+    node->with_sum = residual.defined(), node->with_weight = weight.defined();
+    if (weight.defined()) node->weight_ = ag::SavedVariable(weight, false);
+    ag::set_history(out, node);
+    if (residual.defined()) {
+      ag::set_history(sum, node);
+      node->rows_ = ag::SavedVariable(sum, true);
+    } else {
+      node->rows_ = ag::SavedVariable(rows, false);
+    }
+  }
+  const int parts = 1 + quantized + residual.defined();
+  if (parts == 1) return THPVariable_Wrap(std::move(out));
+  PyObject *made = PyTuple_New(parts);
+  int at_ = 0;
+  PyTuple_SET_ITEM(made, at_++, THPVariable_Wrap(std::move(out)));
+  if (quantized) PyTuple_SET_ITEM(made, at_++, THPVariable_Wrap(std::move(scale)));
+  if (residual.defined()) PyTuple_SET_ITEM(made, at_++, THPVariable_Wrap(std::move(sum)));
+  return made;
+  SCN_END
+}
+
 // (check function): how a failing status becomes an exception
 SCN_FN(set_check) {
   SCN_BEGIN(1)
@@ -1077,7 +1227,8 @@ PyMethodDef methods[] = {
     SCN_METHOD(pooling_forward),         SCN_METHOD(pooling_backward),   SCN_METHOD(sparse_to_dense),
     SCN_METHOD(active_sites),            SCN_METHOD(strided_size),       SCN_METHOD(transposed_size),
     SCN_METHOD(convolution_train),       SCN_METHOD(batchnorm_train),    SCN_METHOD(pooling_train),
-    SCN_METHOD(strided_chain_start),     SCN_METHOD(rows_affine_train),       SCN_METHOD(input_layer),             SCN_METHOD(versions),           SCN_METHOD(set_check),                    {nullptr, nullptr, 0, nullptr}};
+    SCN_METHOD(strided_chain_start),     SCN_METHOD(rows_affine_train),       SCN_METHOD(input_layer),             SCN_METHOD(versions),           SCN_METHOD(set_check),
+    SCN_METHOD(rms_norm),                {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -14,7 +14,7 @@ import torch
 from torch.nn import Module, Parameter
 
 import sparseconvnet_b200 as _pkg
-from . import SCN, autograd
+from . import SCN, autograd, rows
 from .sparse_tensor import SparseConvNetTensor, optional_tensor, to_long_tensor
 
 
@@ -507,6 +507,49 @@ class BatchNormLeakyReLU(BatchNormalization):
     def __repr__(self):
         return "BatchNormLeakyReLU(%d,eps=%g,momentum=%g,affine=%s,leakiness=%g)" % (
             self.nPlanes, self.eps, self.momentum, self.affine, self.leakiness)
+
+
+class RMSNormalization(Module):
+    """Root-mean-square norm of every site's planes: x / sqrt(mean(x^2) + eps) * weight.  Unlike BatchNormalization it needs no
+    other site: no statistics, the same in training and evaluation.  Not in the reference."""
+
+    def __init__(self, nPlanes, eps=1e-6, affine=True):
+        Module.__init__(self)
+        self.nPlanes = nPlanes
+        self.eps = eps
+        self.affine = affine
+        if affine:
+            self.weight = Parameter(torch.ones(nPlanes))
+
+    def forward(self, input):
+        if input.features.nelement() == 0:
+            return input
+        assert input.features.size(1) == self.nPlanes, (self.nPlanes, input.features.shape)
+        output = SparseConvNetTensor(metadata=input.metadata, spatial_size=input.spatial_size)
+        output.features = rows.rms_norm(input.features, parameter(self, "weight"), eps=self.eps)
+        return output
+
+    def input_spatial_size(self, out_size):
+        return out_size
+
+    def __repr__(self):
+        return "%s(%d,eps=%g,affine=%s)" % (type(self).__name__, self.nPlanes, self.eps, self.affine)
+
+
+class AddRMSNormalization(RMSNormalization):
+    """An AddTable and an RMSNormalization in one pass.  Takes a list of two tensors over the same sites, a branch and the
+    residual, and returns the list [norm of the sum, sum]: the sum goes on as the next block's residual."""
+
+    def forward(self, input):
+        branch, residual = input
+        assert branch.features.nelement() == 0 or branch.features.size(1) == self.nPlanes, (self.nPlanes, branch.features.shape)
+        norm, total = (SparseConvNetTensor(metadata=branch.metadata, spatial_size=branch.spatial_size) for _ in range(2))
+        if branch.features.nelement() == 0:
+            norm.features, total.features = branch.features, residual.features
+            return [norm, total]
+        norm.features, total.features = rows.rms_norm(branch.features, parameter(self, "weight"), residual=residual.features,
+                                                      eps=self.eps)
+        return [norm, total]
 
 
 class MaxPooling(Module):
