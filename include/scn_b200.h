@@ -654,6 +654,28 @@ SCN_API int scn_rms_norm_backward(const void *s, int64_t s_stride, int type, con
                                   const void *d_out, int d_out_type, const void *d_sum, int64_t n_rows, int n_planes,
                                   void *d_x, float *d_weight, void *stream);
 
+/* One step of AdamW (decoupled weight decay) over a list of tensors, in place:
+ *     t = *step + 1      m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2
+ *     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * `tensors` is a HOST array; it is read during the call.  step: DEVICE word, the steps done so far (below 2^40), one more
+ * when the work is done.  lr_dev (DEVICE, may be NULL) takes lr's place, so that a replayed graph can follow a schedule.
+ * state_bits 32: exp_avg = m and exp_avg_sq = v, float32.  state_bits 8: e4m3 values of m and of sqrt(v), which stand for
+ * value * scale of their block of 256 values (scales: ceil(n / 256) floats each); rounded to a neighbour by chance in
+ * proportion to the distance, by bits that depend on seed, step and the value's place in the list, where each tensor takes
+ * whole blocks.  copy_type -1, or the type in which `copy` receives the new parameters as well.  The tensors of a list must
+ * not overlap; two calls with the same `step` word must not run at once. */
+typedef struct scn_adamw_tensor {
+  void *param;
+  const void *grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale; /* state_bits 8 */
+  void *copy;                              /* NULL without copies */
+  int64_t n;
+} scn_adamw_tensor;
+SCN_API int scn_adamw_step(const scn_adamw_tensor *tensors, int64_t n_tensors, int param_type, int grad_type, int state_bits,
+                           int copy_type, int64_t *step, double lr, const float *lr_dev, double beta1, double beta2, double eps,
+                           double weight_decay, uint32_t seed, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,3 +45,4 @@ from .layers import (InputLayer, OutputLayer, BLInputLayer, BLOutputLayer, Subma
 from .rows import rms_norm, rms_norm_quantized  # noqa: E402
 from .containers import Sequential, ConcatTable, JoinTable, AddTable  # noqa: E402
 from .architectures import SparseVggNet, SparseResNet, UNet, FullyConvolutionalNet  # noqa: E402
+from .optim import AdamW, adamw_step  # noqa: E402

@@ -68,6 +68,8 @@ SIGNATURES = {
                                             C.POINTER(C.c_double)]),
     "scn_batchnorm_join_forward": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_double,
                                              C.c_double, _vp]),
+    "scn_adamw_step": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_double, _vp, C.c_double,
+                                 C.c_double, C.c_double, C.c_double, C.c_uint32, _vp]),
     "scn_rms_norm_forward": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, C.c_int, _vp, C.c_int64, C.c_int, C.c_double, _vp, _vp,
                                        C.c_int, _vp, _vp, _vp]),
     "scn_rms_norm_backward": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, _vp, _vp,

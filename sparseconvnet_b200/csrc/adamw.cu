@@ -1,0 +1,341 @@
+// One step of AdamW over all tensors of a list, with moments in 32 bits or in 8.
+//
+//     t = steps done + 1     m = b1 m + (1 - b1) g     v = b2 v + (1 - b2) g g
+//     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8 bits: m and r = sqrt(v) as e4m3 with one scale for 256 values (the block's largest / 448); r rather than v, because its
+// range is half as wide in powers of two.  A decay of 0.1% is far below half a step of 8 bits, so rounding to nearest would
+// leave a moment where it is for good: it is rounded up or down by chance, in proportion to the distance, which keeps its
+// mean.  The bits come from a hash of seed, step and position: the same call gives the same bits.  A positive r is never
+// rounded to zero (its value would be divided by eps then).  The step itself uses m and r as computed, in fp32.
+//
+// Bound by HBM: 28 bytes for a value in 32 bits, 16 in 8 (fp32 parameters and gradients).  The list's pointers travel as
+// kernel arguments (no copy to the device, nothing to keep alive for a graph).  A warp takes whole blocks of 256 values, 8 to
+// a lane, and a run of neighbouring blocks, so that it looks for their tensor once; a block's maximum is five shuffles.
+// The count of steps lives on the device, so that a replayed graph counts on: the last block to end adds one to it, and
+// which block that is, is counted in the upper bits of the same word.
+#include <math.h>
+
+#include <algorithm>
+
+#include "rows.cuh"
+
+namespace scn {
+namespace {
+
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kBlock = 256;  // values of a block
+constexpr int kTicketShift = 40;
+constexpr float kSmallest = 1e-30f, kE4m3Most = 448.f, kE4m3Least = 1.f / 512.f;
+
+struct Entry {
+  void *p, *m, *v, *copy;
+  const void *g;
+  float *m_scale, *v_scale;
+  long long n, first;  // values; number of the tensor's first block in the list (lowest bit of `aligned` apart)
+};
+template <int CAP>
+struct Table {
+  Entry e[CAP];
+};
+struct Step {
+  unsigned long long *word;  // steps done; blocks that have ended above bit 40
+  const float *lr_dev;       // may be null
+  double log_b1, log_b2;
+  float lr, b1, b2, one_minus_b1, one_minus_b2, eps, wd;
+  unsigned seed;
+  int grad_type, copy_type;  // copy_type -1: none
+  int count;                 // tensors of this launch
+  int last;                  // of the list's launches: counts the step
+  long long first, blocks;   // this launch's blocks of the list
+};
+
+__device__ __forceinline__ unsigned mixed(unsigned v) {  // the 32-bit finaliser of MurmurHash3
+  v = (v ^ (v >> 16)) * 0x85EBCA6Bu;
+  v = (v ^ (v >> 13)) * 0xC2B2AE35u;
+  return v ^ (v >> 16);
+}
+
+// 16 random bits as a number in [0, 1)
+__device__ __forceinline__ float chance(unsigned bits16) { return __uint_as_float(0x3F800000u | bits16 << 7) - 1.f; }
+
+// |y| <= 448 to one of its two neighbours among the values of e4m3
+__device__ __forceinline__ float to_neighbour(float y, float u) {
+  const unsigned e = max(__float_as_uint(y) & 0x7F800000u, 121u << 23);  // the exponent, at least -6
+  const float per_step = __uint_as_float((257u << 23) - e), step = __uint_as_float(e - (3u << 23));
+  return fminf(floorf(fmaf(fabsf(y), per_step, u)) * step, kE4m3Most);
+}
+
+__device__ __forceinline__ float largest(float v) {  // over the warp; a NaN is above all numbers
+  unsigned b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, b));
+}
+
+__device__ __forceinline__ void from_e4m3(const uint2 q, float scale, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? q.x : q.y) >> (i % 2 * 16)), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    v[2 * i] = f.x * scale, v[2 * i + 1] = f.y * scale;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float one(const void *p, long long i);
+template <>
+__device__ __forceinline__ float one<float>(const void *p, long long i) { return ((const float *)p)[i]; }
+template <>
+__device__ __forceinline__ float one<__nv_bfloat16>(const void *p, long long i) { return __bfloat162float(((const __nv_bfloat16 *)p)[i]); }
+template <>
+__device__ __forceinline__ float one<__half>(const void *p, long long i) { return __half2float(((const __half *)p)[i]); }
+__device__ __forceinline__ void put(float *p, long long i, float v) { p[i] = v; }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, long long i, float v) { p[i] = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half *p, long long i, float v) { p[i] = __float2half_rn(v); }
+
+// 8 values from `at` on (vectors), or the values at + 32 j that lie below n
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void get8(const void *p, long long at, long long n, float (&v)[8]) {
+  if (WHOLE) {
+    unsigned w[Words<T>::N];
+#pragma unroll
+    for (int i = 0; i < Words<T>::N; i += 4) {
+      const uint4 q = load_stream((const unsigned *)((const T *)p + at) + i);
+      w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+    }
+    unpack8(w, v, T());
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = at + 32 * j < n ? one<T>(p, at + 32 * j) : 0.f;
+  }
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void put8(void *p, long long at, long long n, const float (&v)[8]) {
+  if (WHOLE) {
+    unsigned w[Words<T>::N];
+    pack8(v, w, T());
+#pragma unroll
+    for (int i = 0; i < Words<T>::N; i += 4)
+      __stcs(reinterpret_cast<uint4 *>((unsigned *)((T *)p + at) + i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at + 32 * j < n) put((T *)p, at + 32 * j, v[j]);
+  }
+}
+template <bool WHOLE>
+__device__ __forceinline__ void get8_e4m3(const void *p, long long at, long long n, float scale, float (&v)[8]) {
+  const unsigned char *b = (const unsigned char *)p;
+  uint2 q;
+  if (WHOLE) {
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(b + at));
+  } else {
+    unsigned c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = at + 32 * j < n ? b[at + 32 * j] : 0u;
+    q = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+  }
+  from_e4m3(q, scale, v);
+}
+template <bool WHOLE>
+__device__ __forceinline__ void put8_e4m3(void *p, long long at, long long n, const float (&v)[8]) {
+  unsigned char *b = (unsigned char *)p;
+  const uint2 q = make_uint2(e4m3_pair(v[0], v[1]) | e4m3_pair(v[2], v[3]) << 16, e4m3_pair(v[4], v[5]) | e4m3_pair(v[6], v[7]) << 16);
+  if (WHOLE) {
+    __stcs(reinterpret_cast<uint2 *>(b + at), q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at + 32 * j < n) b[at + 32 * j] = (unsigned char)((j < 4 ? q.x : q.y) >> (j % 4 * 8));
+  }
+}
+
+// One block of 256 values: block `number` of the list, `at` of its tensor
+template <typename P, int BITS, bool WHOLE>
+__device__ __forceinline__ void one_block(const Entry &E, const Step &A, long long at, long long number, unsigned key, float rate,
+                                          float per_root, int lane) {
+  const long long first = at * kBlock + (WHOLE ? lane * 8 : lane);
+  float p[8], g[8], m[8], r[8];
+  get8<P, WHOLE>(E.p, first, E.n, p);
+  if (A.grad_type == SCN_TYPE_FLOAT32)
+    get8<float, WHOLE>(E.g, first, E.n, g);
+  else if (A.grad_type == SCN_TYPE_BFLOAT16)
+    get8<__nv_bfloat16, WHOLE>(E.g, first, E.n, g);
+  else
+    get8<__half, WHOLE>(E.g, first, E.n, g);
+  if (BITS == 8) {
+    get8_e4m3<WHOLE>(E.m, first, E.n, E.m_scale[at], m);
+    get8_e4m3<WHOLE>(E.v, first, E.n, E.v_scale[at], r);
+  } else {
+    get8<float, WHOLE>(E.m, first, E.n, m);
+    get8<float, WHOLE>(E.v, first, E.n, r);
+  }
+  const float keep = 1.f - A.wd;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {  // (the roundings of the formula as it is written: no contraction)
+    const float v = BITS == 8 ? __fmul_rn(r[j], r[j]) : r[j];
+    m[j] = __fadd_rn(__fmul_rn(m[j], A.b1), __fmul_rn(g[j], A.one_minus_b1));
+    const float now = __fadd_rn(__fmul_rn(v, A.b2), __fmul_rn(__fmul_rn(g[j], g[j]), A.one_minus_b2));
+    const float root = __fsqrt_rn(now);
+    p[j] = fmaf(-rate, __fdividef(m[j], fmaf(root, per_root, A.eps)), p[j] * keep);
+    r[j] = BITS == 8 ? root : now;
+  }
+  put8<P, WHOLE>(E.p, first, E.n, p);
+  if (A.copy_type == SCN_TYPE_BFLOAT16)
+    put8<__nv_bfloat16, WHOLE>(E.copy, first, E.n, p);
+  else if (A.copy_type == SCN_TYPE_FLOAT16)
+    put8<__half, WHOLE>(E.copy, first, E.n, p);
+  if (BITS == 32) {
+    put8<float, WHOLE>(E.m, first, E.n, m);
+    put8<float, WHOLE>(E.v, first, E.n, r);
+    return;
+  }
+  float most_m = 0.f, most_r = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    most_m = __uint_as_float(max(__float_as_uint(most_m), __float_as_uint(m[j]) & 0x7FFFFFFFu));
+    most_r = __uint_as_float(max(__float_as_uint(most_r), __float_as_uint(r[j]) & 0x7FFFFFFFu));
+  }
+  most_m = __uint_as_float(max(__float_as_uint(largest(most_m)), __float_as_uint(kSmallest)));
+  most_r = __uint_as_float(max(__float_as_uint(largest(most_r)), __float_as_uint(kSmallest)));
+  if (lane == 0) {
+    E.m_scale[at] = __fmul_rn(most_m, 1.f / kE4m3Most);
+    E.v_scale[at] = __fmul_rn(most_r, 1.f / kE4m3Most);
+  }
+  const float per_m = __fmul_rn(__frcp_rn(most_m), kE4m3Most), per_r = __fmul_rn(__frcp_rn(most_r), kE4m3Most);
+  const unsigned low = (unsigned)(number * kBlock), high = (unsigned)(number * kBlock >> 32);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned bits = mixed(mixed((low + (WHOLE ? lane * 8 + j : lane + 32 * j)) ^ key) ^ high);
+    const float ym = __fmul_rn(m[j], per_m), yr = __fmul_rn(r[j], per_r);
+    m[j] = copysignf(to_neighbour(ym, chance(bits & 0xFFFFu)), ym);
+    r[j] = to_neighbour(yr, chance(bits >> 16));
+    if (yr > 0.f) r[j] = fmaxf(r[j], kE4m3Least);
+    if (isnan(ym)) m[j] = ym;  // (the smaller of a NaN and 448 is 448)
+    if (isnan(yr)) r[j] = yr;
+  }
+  put8_e4m3<WHOLE>(E.m, first, E.n, m);
+  put8_e4m3<WHOLE>(E.v, first, E.n, r);
+}
+
+template <typename P, int BITS, int CAP>
+__global__ void __launch_bounds__(kThreads)
+k_adamw(const __grid_constant__ Table<CAP> T, const __grid_constant__ Step A) {
+  SCN_GRID_WAIT();
+  const int lane = threadIdx.x % 32;
+  const unsigned long long mask = (1ull << kTicketShift) - 1;
+  const unsigned long long done = *(volatile unsigned long long *)A.word & mask;
+  const double t = (double)(done + 1);
+  // 1 - b^t by expm1 of its logarithm: exact to fp32 for the first steps and for b near one alike
+  const float bc1 = -expm1f((float)(t * A.log_b1)), bc2 = -expm1f((float)(t * A.log_b2));
+  const float lr = A.lr_dev ? *A.lr_dev : A.lr;
+  const float rate = lr / bc1, per_root = 1.f / sqrtf(bc2);
+  const unsigned key = mixed((unsigned)(done + 1) * 0x9E3779B1u + A.seed);
+  const long long warps = (long long)gridDim.x * kWarps, warp = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
+  const long long share = A.blocks / warps, extra = A.blocks % warps;
+  long long b = A.first + warp * share + min(warp, extra);
+  const long long end = b + share + (warp < extra);
+  Step B = A;
+  B.wd = lr * A.wd;
+  if (b < end) {
+    int lo = 0, hi = A.count - 1;  // the last tensor that begins at or before b and is not empty there
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (T.e[mid].first >> 1 <= b)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    for (; b < end; ++b) {
+      while (lo + 1 < A.count && T.e[lo + 1].first >> 1 <= b) ++lo;
+      const Entry &E = T.e[lo];
+      const long long at = b - (E.first >> 1);
+      if ((E.first & 1) && (at + 1) * kBlock <= E.n)
+        one_block<P, BITS, true>(E, B, at, b, key, rate, per_root, lane);
+      else
+        one_block<P, BITS, false>(E, B, at, b, key, rate, per_root, lane);
+    }
+  }
+  if (!A.last) return;
+  __syncthreads();  // (every warp has read the word)
+  if (threadIdx.x == 0) {
+    const unsigned long long was = atomicAdd(A.word, 1ull << kTicketShift);
+    if (was >> kTicketShift == gridDim.x - 1) atomicAdd(A.word, 1ull - ((unsigned long long)gridDim.x << kTicketShift));
+  }
+}
+
+template <typename P, int BITS, int CAP>
+int launch(const scn_adamw_tensor *tensors, int64_t n, Step A, cudaStream_t stream) {
+  auto blocks_of = [](int64_t values) { return ceil_div(values, kBlock); };
+  long long first = 0;
+  int64_t i = 0;
+  do {
+    Table<CAP> T;
+    A.count = 0;
+    A.first = first;
+    for (; i < n && A.count < CAP; ++i) {
+      const scn_adamw_tensor &t = tensors[i];
+      if (t.n == 0) continue;
+      bool aligned = true;
+      for (const void *p : {(const void *)t.param, t.grad, (const void *)t.exp_avg, (const void *)t.exp_avg_sq, (const void *)t.copy})
+        aligned = aligned && (uintptr_t)p % 16 == 0;
+      T.e[A.count++] = {t.param, t.exp_avg, t.exp_avg_sq, t.copy, t.grad, t.exp_avg_scale, t.exp_avg_sq_scale, t.n, first * 2 + aligned};
+      first += blocks_of(t.n);
+    }
+    A.blocks = first - A.first;
+    A.last = i == n;
+    int most = 0;
+    SCN_TRY((resident_blocks<k_adamw<P, BITS, CAP>>(kThreads, 0, &most)));
+    const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(most, ceil_div(A.blocks, kWarps)));
+    SCN_LAUNCH((k_adamw<P, BITS, CAP>), grid, kThreads, 0, stream, T, A);
+    SCN_CUDA_CHECK(cudaGetLastError());
+  } while (i < n);
+  return SCN_OK;
+}
+
+// Few tensors take a short table: 32 KB of arguments cost the launch some microseconds.
+constexpr int kFew = 48, kMany = 440;
+template <typename P, int BITS>
+int launch_list(const scn_adamw_tensor *tensors, int64_t n, const Step &A, cudaStream_t stream) {
+  return n <= kFew ? launch<P, BITS, kFew>(tensors, n, A, stream) : launch<P, BITS, kMany>(tensors, n, A, stream);
+}
+
+}  // namespace
+}  // namespace scn
+
+using namespace scn;
+
+extern "C" int scn_adamw_step(const scn_adamw_tensor *tensors, int64_t n_tensors, int param_type, int grad_type, int state_bits,
+                              int copy_type, int64_t *step, double lr, const float *lr_dev, double beta1, double beta2, double eps,
+                              double weight_decay, uint32_t seed, void *stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  auto is_type = [](int t) { return t == SCN_TYPE_FLOAT32 || t == SCN_TYPE_BFLOAT16 || t == SCN_TYPE_FLOAT16; };
+  SCN_REQUIRE(is_type(param_type) && is_type(grad_type), SCN_ERR_BAD_ARG, "adamw_step: unknown type");
+  SCN_REQUIRE(copy_type == -1 || copy_type == SCN_TYPE_BFLOAT16 || copy_type == SCN_TYPE_FLOAT16, SCN_ERR_BAD_ARG,
+              "adamw_step: copies are bfloat16 or float16");
+  SCN_REQUIRE(state_bits == 8 || state_bits == 32, SCN_ERR_BAD_ARG, "adamw_step: states have 8 or 32 bits");
+  SCN_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, SCN_ERR_BAD_ARG, "adamw_step: betas must lie in [0, 1)");
+  SCN_REQUIRE(eps >= 0 && weight_decay >= 0 && (lr_dev || lr >= 0), SCN_ERR_BAD_ARG,
+              "adamw_step: lr, eps and weight_decay must not be negative");
+  SCN_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || tensors) && step, SCN_ERR_BAD_ARG, "adamw_step: null argument");
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    const scn_adamw_tensor &t = tensors[i];
+    SCN_REQUIRE(t.n >= 0, SCN_ERR_BAD_ARG, "adamw_step: bad size");
+    if (t.n == 0) continue;
+    SCN_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq && (state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale)) &&
+                    (copy_type == -1) == (t.copy == nullptr),
+                SCN_ERR_BAD_ARG, "adamw_step: null argument");
+  }
+  Step A{};
+  A.word = (unsigned long long *)step;
+  A.lr_dev = lr_dev;
+  // (b = 0 has no logarithm: 1 - 0^t = 1, which expm1 of a large negative number is too)
+  A.log_b1 = beta1 > 0 ? log(beta1) : -1e4;
+  A.log_b2 = beta2 > 0 ? log(beta2) : -1e4;
+  A.lr = (float)lr, A.b1 = (float)beta1, A.b2 = (float)beta2;
+  A.one_minus_b1 = (float)(1 - beta1), A.one_minus_b2 = (float)(1 - beta2);
+  A.eps = (float)eps, A.wd = (float)weight_decay;
+  A.seed = seed, A.grad_type = grad_type, A.copy_type = copy_type;
+#define SCN_BY_BITS(P) (state_bits == 8 ? launch_list<P, 8>(tensors, n_tensors, A, stream) : launch_list<P, 32>(tensors, n_tensors, A, stream))
+  return param_type == SCN_TYPE_FLOAT32 ? SCN_BY_BITS(float) : param_type == SCN_TYPE_BFLOAT16 ? SCN_BY_BITS(__nv_bfloat16) : SCN_BY_BITS(__half);
+#undef SCN_BY_BITS
+}

@@ -1210,6 +1210,109 @@ SCN_FN(rms_norm) {
   SCN_END
 }
 
+struct List {  // a sequence of tensors, or None
+  PyObject *seq = nullptr;
+  Py_ssize_t n = 0;
+  const char *name;
+  List(PyObject *o, const char *what, Py_ssize_t expected = -1) : name(what) {
+    if (o == Py_None) return;
+    seq = PySequence_Fast(o, "a list of tensors is expected");
+    if (!seq) throw Fail{};
+    n = PySequence_Fast_GET_SIZE(seq);
+    if (expected >= 0 && n != expected) {
+      Py_CLEAR(seq);
+      fail("%s has %lld tensors, params %lld", name, (long long)n, (long long)expected);
+    }
+  }
+  List(const List &) = delete;
+  ~List() { Py_XDECREF(seq); }
+  const at::Tensor &at(Py_ssize_t i) const { return on_gpu(PySequence_Fast_GET_ITEM(seq, i), name); }
+};
+
+// written in place by the library
+void *written(const at::Tensor &t, at::ScalarType type, const at::Tensor &like, int64_t n, const char *name) {
+  if (t.scalar_type() != type) fail("%s: %s expected, got %s", name, at::toString(type), at::toString(t.scalar_type()));
+  if (t.numel() != n) fail("%s: %lld values expected, got %lld", name, (long long)n, (long long)t.numel());
+  if (t.device() != like.device()) fail("%s is on another device than the first parameter", name);
+  if (!t.is_contiguous()) fail("%s must be contiguous", name);
+  return raw(t);
+}
+
+// (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales or None, exp_avg_sq_scales or None, copies or None, step, lr, beta1,
+//  beta2, eps, weight_decay, seed) -> None
+SCN_FN(adamw_step) {
+  SCN_BEGIN(14)
+  const List params(a[0], "params"), grads(a[1], "grads", params.n), m(a[2], "exp_avgs", params.n), v(a[3], "exp_avg_sqs", params.n),
+      ms(a[4], "exp_avg_scales", params.n), vs(a[5], "exp_avg_sq_scales", params.n), copies(a[6], "copies", params.n);
+  if (!params.seq || !grads.seq || !m.seq || !v.seq) fail("params, grads, exp_avgs and exp_avg_sqs must be lists of tensors");
+  const at::Tensor &step = on_gpu(a[7], "step");
+  float *lr_dev = nullptr;
+  double lr = 0;
+  if (THPVariable_Check(a[8])) {
+    const at::Tensor &t = on_gpu(a[8], "lr");
+    lr_dev = (float *)written(t, at::kFloat, step, 1, "lr");
+  } else {
+    lr = PyFloat_AsDouble(a[8]);
+  }
+  const double beta1 = PyFloat_AsDouble(a[9]), beta2 = PyFloat_AsDouble(a[10]), eps = PyFloat_AsDouble(a[11]), wd = PyFloat_AsDouble(a[12]);
+  const unsigned long seed = PyLong_AsUnsignedLongMask(a[13]);
+  if (PyErr_Occurred()) throw Fail{};
+  if ((ms.seq == nullptr) != (vs.seq == nullptr)) fail("scales come for both moments or for none");
+  const at::ScalarType param_type = params.n ? params.at(0).scalar_type() : at::kFloat, grad_type = params.n ? grads.at(0).scalar_type() : at::kFloat;
+  const int param_code = params.n ? type_of(params.at(0), "params") : 0, grad_code = params.n ? type_of(grads.at(0), "grads") : 0;
+  const int bits = ms.seq ? 8 : 32;
+  const at::ScalarType state_type = ms.seq ? at::kFloat8_e4m3fn : at::kFloat;
+  at::ScalarType copy_type = at::kBFloat16;
+  int copy_code = -1;
+  if (copies.seq && params.n) {
+    copy_type = copies.at(0).scalar_type();
+    copy_code = type_of(copies.at(0), "copies");
+    if (copy_code == SCN_TYPE_FLOAT32) fail("copies must be bfloat16 or float16");
+  }
+  int64_t *word = (int64_t *)written(step, at::kLong, step, 1, "step");
+  std::vector<scn_adamw_tensor> table((size_t)params.n);
+  std::vector<at::Tensor> held, touched;
+  std::vector<void *> seen;
+  for (Py_ssize_t i = 0; i < params.n; ++i) {
+    scn_adamw_tensor &e = table[(size_t)i];
+    const at::Tensor &p = params.at(i), &g = grads.at(i);
+    const int64_t n = e.n = p.numel(), blocks = (n + 255) / 256;
+    e.param = written(p, param_type, step, n, "params");
+    if (g.scalar_type() != grad_type || g.sizes() != p.sizes() || g.device() != step.device())
+      fail("grads must have the shapes of params, one type, and their device");
+    held.push_back(g.is_contiguous() ? g : g.contiguous());
+    e.grad = raw(held.back());
+    e.exp_avg = written(m.at(i), state_type, step, n, "exp_avgs");
+    e.exp_avg_sq = written(v.at(i), state_type, step, n, "exp_avg_sqs");
+    touched.insert(touched.end(), {p, m.at(i), v.at(i)});
+    e.exp_avg_scale = e.exp_avg_sq_scale = nullptr;
+    if (ms.seq) {
+      e.exp_avg_scale = (float *)written(ms.at(i), at::kFloat, step, blocks, "exp_avg_scales");
+      e.exp_avg_sq_scale = (float *)written(vs.at(i), at::kFloat, step, blocks, "exp_avg_sq_scales");
+      touched.insert(touched.end(), {ms.at(i), vs.at(i)});
+    }
+    e.copy = nullptr;
+    if (copy_code >= 0) {
+      e.copy = written(copies.at(i), copy_type, step, n, "copies");
+      touched.push_back(copies.at(i));
+    }
+  }
+  for (const at::Tensor &t : touched)
+    if (t.numel()) seen.push_back(t.data_ptr());
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) fail("a tensor is in the lists twice");
+  {
+    const OnDevice on(step);
+    SCN_CALL(scn_adamw_step(table.data(), (int64_t)params.n, param_code, grad_code, bits, copy_code, word, lr, lr_dev, beta1, beta2,
+                            eps, wd, (uint32_t)seed, on.stream));
+  }
+  touched.push_back(step);
+  for (const at::Tensor &t : touched)  // whoever keeps something by a tensor's version sees that it was written
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  Py_RETURN_NONE;
+  SCN_END
+}
+
 // (check function): how a failing status becomes an exception
 SCN_FN(set_check) {
   SCN_BEGIN(1)
@@ -1228,7 +1331,7 @@ PyMethodDef methods[] = {
     SCN_METHOD(active_sites),            SCN_METHOD(strided_size),       SCN_METHOD(transposed_size),
     SCN_METHOD(convolution_train),       SCN_METHOD(batchnorm_train),    SCN_METHOD(pooling_train),
     SCN_METHOD(strided_chain_start),     SCN_METHOD(rows_affine_train),       SCN_METHOD(input_layer),             SCN_METHOD(versions),           SCN_METHOD(set_check),
-    SCN_METHOD(rms_norm),                {nullptr, nullptr, 0, nullptr}};
+    SCN_METHOD(rms_norm),                SCN_METHOD(adamw_step),         {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,127 @@
+"""AdamW over all parameters of a network in one kernel, moments in 32 bits or in 8.
+
+``adamw_step`` is the step on plain lists of tensors, ``AdamW`` the torch optimizer around it.  Stands beside the
+data-parallel helpers of ``shard.py``: ``shard.sum_gradients(parameters)`` and then ``optimizer.step()``."""
+import torch
+
+from . import SCN
+
+BLOCK = 256  # values of a block that shares a scale, in 8-bit moments
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               exp_avg_scales=None, exp_avg_sq_scales=None, seed=0, copies=None):
+    """One step, in place, over lists of contiguous CUDA tensors of one type each:
+
+        m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2        t = step + 1
+        p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+
+    params, grads: float32, bfloat16 or float16 (each list one type).  step: int64 CUDA tensor of one value, the steps done
+    so far; it is advanced on the device, so a captured step counts on when it is replayed.  lr: a number, or a float32
+    CUDA tensor of one value that is read when the step runs.
+
+    exp_avgs, exp_avg_sqs: float32 m and v.  With the scales (float32, one per block of 256 values): float8_e4m3fn m and
+    sqrt(v), which stand for value * scale of the block; they are rounded by chance in proportion to the distance of the two
+    neighbours, with bits that depend on seed, step and place only, so a run can be repeated.  A gradient that is no
+    number makes its value's moments NaN, in 8 bits those of its block.
+    copies: bfloat16 or float16 tensors that receive the new parameters as well.
+
+    All work is queued on the current stream.  The call refuses lists in which a tensor occurs twice; tensors that overlap in
+    other ways must not be passed."""
+    SCN._binding.adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, copies, step, lr,
+                            betas[0], betas[1], eps, weight_decay, seed)
+
+
+def _state_of(p, bits):
+    if bits == 32:
+        return {"exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device),
+                "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
+    blocks = -(-p.numel() // BLOCK)
+    made = {}
+    for k in ("exp_avg", "exp_avg_sq"):
+        made[k] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+        made[k + "_scale"] = torch.zeros(blocks, device=p.device)
+    return made
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update on the GPU in one launch for all parameters of a group.
+
+    state_bits: 32, or 8 for moments of 8 bits with a scale per 256 values (2.03 bytes a value instead of 8).
+    master_weights: for bfloat16 / float16 parameters, keep them in float32 as well and round the parameters from those;
+    without it an update smaller than half a step of the parameter's type is lost.
+    lr of a group may be a float32 CUDA tensor of one value.  Parameters without a gradient are left as they are, and their
+    step is not counted.  There is no amsgrad, no maximize and no CPU path."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError("lr must not be negative")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("betas must lie in [0, 1)")
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError("eps and weight_decay must not be negative")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, seed=seed))
+
+    def _start(self, p, group):
+        state = _state_of(p, group["state_bits"])
+        if group["master_weights"] and p.dtype != torch.float32:
+            state["master"] = p.detach().float()
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for number, group in enumerate(self.param_groups):
+            fresh = {}    # device -> the counter of parameters that take their first step now
+            together = {}  # parameters that step as one list: one counter, one device, one type
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                state = self.state[p]
+                if not state:
+                    state.update(self._start(p, group))
+                    if p.device not in fresh:
+                        fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
+                    state["step"] = fresh[p.device]
+                together.setdefault((id(state["step"]), p.dtype, p.grad.dtype, "master" in state), []).append(p)
+            self._one_counter_per_list(group, together)
+            for (_, _, _, master), ps in together.items():
+                states = [self.state[p] for p in ps]
+                column = lambda k: [s[k] for s in states] if k in states[0] else None  # noqa: E731
+                adamw_step(column("master") if master else ps, [p.grad for p in ps], column("exp_avg"), column("exp_avg_sq"),
+                           states[0]["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                           column("exp_avg_scale"), column("exp_avg_sq_scale"), group["seed"] + number, ps if master else None)
+        return loss
+
+    def _one_counter_per_list(self, group, together):
+        """A counter is advanced by the one list that has it: parameters that share it but step in another list, or not at all
+        this time, keep the old count in a counter of their own."""
+        users = {}
+        for p in group["params"]:
+            if self.state.get(p):
+                users.setdefault(id(self.state[p]["step"]), []).append(p)
+        for key, ps in together.items():
+            if len(users[key[0]]) > len(ps):
+                own = self.state[ps[0]]["step"].clone()
+                for p in ps:
+                    self.state[p]["step"] = own
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but states keep their types (torch casts them to the parameter's), and parameters with the same count
+        share a counter again."""
+        super().load_state_dict(state_dict)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            counters = {}
+            for i, p in zip(saved["params"], group["params"]):
+                if i in state_dict["state"]:
+                    state = {k: v.to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
+                    state["step"] = counters.setdefault((int(state["step"]), p.device), state["step"])
+                    self.state[p] = state
