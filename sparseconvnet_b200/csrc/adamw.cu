@@ -11,7 +11,7 @@
 //
 // Bound by HBM: 28 bytes for a value in 32 bits, 16 in 8 (fp32 parameters and gradients).  The list's pointers travel as
 // kernel arguments (no copy to the device, nothing to keep alive for a graph).  A warp takes whole blocks of 256 values, 8 to
-// a lane, and a run of neighbouring blocks, so that it looks for their tensor once; a block's maximum is five shuffles.
+// a lane, and looks for a block's tensor from the one before on; a block's maximum is one reduction over the warp.
 // The count of steps lives on the device, so that a replayed graph counts on: the last block to end adds one to it, and
 // which block that is, is counted in the upper bits of the same word.
 #include <math.h>
@@ -59,16 +59,21 @@ __device__ __forceinline__ unsigned mixed(unsigned v) {  // the 32-bit finaliser
 // 16 random bits as a number in [0, 1)
 __device__ __forceinline__ float chance(unsigned bits16) { return __uint_as_float(0x3F800000u | bits16 << 7) - 1.f; }
 
-// |y| <= 448 to one of its two neighbours among the values of e4m3
+// |y| <= 448 (and what rounding adds) to the multiple of its binade's step below |y| + u step, u < 1: one of its two neighbours
+// among the values of e4m3.  The addition of 2^23 steps, rounded down, drops what lies below a step.
 __device__ __forceinline__ float to_neighbour(float y, float u) {
   const unsigned e = max(__float_as_uint(y) & 0x7F800000u, 121u << 23);  // the exponent, at least -6
-  const float per_step = __uint_as_float((257u << 23) - e), step = __uint_as_float(e - (3u << 23));
-  return fminf(floorf(fmaf(fabsf(y), per_step, u)) * step, kE4m3Most);
+  const float step = __uint_as_float(e - (3u << 23)), steps = __uint_as_float(e + (20u << 23));
+  return __fadd_rd(fmaf(u, step, fabsf(y)), steps) - steps;
 }
 
-__device__ __forceinline__ float largest(float v) {  // over the warp; a NaN is above all numbers
-  unsigned b = __float_as_uint(v) & 0x7FFFFFFFu;
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, b));
+__device__ __forceinline__ float larger(float a, float b) {  // max(a, |b|); a NaN is above all numbers
+  float r;
+  asm("{.reg .f32 t; abs.f32 t, %2; max.NaN.f32 %0, %1, t;}" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float largest(float v) {  // over the warp, v >= 0 or NaN
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
 
 __device__ __forceinline__ void from_e4m3(const uint2 q, float scale, float (&v)[8]) {
@@ -176,7 +181,9 @@ __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long lo
     m[j] = __fadd_rn(__fmul_rn(m[j], A.b1), __fmul_rn(g[j], A.one_minus_b1));
     const float now = __fadd_rn(__fmul_rn(v, A.b2), __fmul_rn(__fmul_rn(g[j], g[j]), A.one_minus_b2));
     const float root = __fsqrt_rn(now);
-    p[j] = fmaf(-rate, __fdividef(m[j], fmaf(root, per_root, A.eps)), p[j] * keep);
+    float per;  // (1 / x to a unit in the last place; eps keeps x above the subnormal numbers)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per) : "f"(fmaf(root, per_root, A.eps)));
+    p[j] = fmaf(-rate * m[j], per, p[j] * keep);
     r[j] = BITS == 8 ? root : now;
   }
   put8<P, WHOLE>(E.p, first, E.n, p);
@@ -192,8 +199,8 @@ __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long lo
   float most_m = 0.f, most_r = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    most_m = __uint_as_float(max(__float_as_uint(most_m), __float_as_uint(m[j]) & 0x7FFFFFFFu));
-    most_r = __uint_as_float(max(__float_as_uint(most_r), __float_as_uint(r[j]) & 0x7FFFFFFFu));
+    most_m = larger(most_m, m[j]);
+    most_r = larger(most_r, r[j]);
   }
   most_m = __uint_as_float(max(__float_as_uint(largest(most_m)), __float_as_uint(kSmallest)));
   most_r = __uint_as_float(max(__float_as_uint(largest(most_r)), __float_as_uint(kSmallest)));
@@ -210,8 +217,6 @@ __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long lo
     m[j] = copysignf(to_neighbour(ym, chance(bits & 0xFFFFu)), ym);
     r[j] = to_neighbour(yr, chance(bits >> 16));
     if (yr > 0.f) r[j] = fmaxf(r[j], kE4m3Least);
-    if (isnan(ym)) m[j] = ym;  // (the smaller of a NaN and 448 is 448)
-    if (isnan(yr)) r[j] = yr;
   }
   put8_e4m3<WHOLE>(E.m, first, E.n, m);
   put8_e4m3<WHOLE>(E.v, first, E.n, r);
@@ -231,9 +236,9 @@ k_adamw(const __grid_constant__ Table<CAP> T, const __grid_constant__ Step A) {
   const float rate = lr / bc1, per_root = 1.f / sqrtf(bc2);
   const unsigned key = mixed((unsigned)(done + 1) * 0x9E3779B1u + A.seed);
   const long long warps = (long long)gridDim.x * kWarps, warp = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  const long long share = A.blocks / warps, extra = A.blocks % warps;
-  long long b = A.first + warp * share + min(warp, extra);
-  const long long end = b + share + (warp < extra);
+  // Neighbouring blocks go to neighbouring warps at the same time: DRAM sees seven streams, not seven for every warp.
+  long long b = A.first + warp;
+  const long long end = A.first + A.blocks;
   Step B = A;
   B.wd = lr * A.wd;
   if (b < end) {
@@ -245,7 +250,7 @@ k_adamw(const __grid_constant__ Table<CAP> T, const __grid_constant__ Step A) {
       else
         hi = mid - 1;
     }
-    for (; b < end; ++b) {
+    for (; b < end; b += warps) {
       while (lo + 1 < A.count && T.e[lo + 1].first >> 1 <= b) ++lo;
       const Entry &E = T.e[lo];
       const long long at = b - (E.first >> 1);
