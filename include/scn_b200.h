@@ -676,6 +676,32 @@ SCN_API int scn_adamw_step(const scn_adamw_tensor *tensors, int64_t n_tensors, i
                            int copy_type, int64_t *step, double lr, const float *lr_dev, double beta1, double beta2, double eps,
                            double weight_decay, uint32_t seed, void *stream);
 
+/* Products of ragged groups of rows, each with its group's own weights: for the rows offsets[g] <= r < offsets[g + 1]
+ *     out[r] = x[r] weight[g] (+ bias[g])          weight [n_groups][n_in][n_out], bias [n_groups][n_out] or NULL
+ * and zeros for rows of no group.  offsets [n_groups + 1]: DEVICE int64 (offsets_64 != 0) or int32, not decreasing, within
+ * [0, n_rows]; they are clamped to that, and rows of groups that overlap all the same are undefined.  At most 1024 groups.
+ * 16-bit operands are multiplied as they are, float32 ones according to `precision` (an scn_precision): FP32 as three bf16
+ * parts and six products, TF32 and TF32X3 as two parts and three, BF16 as one.  Sums are float32.  In float32 an infinity
+ * may become NaN (FP32, TF32X3, TF32). */
+SCN_API int scn_grouped_product_forward(const void *x, int64_t x_stride, int type, const void *weight, const void *bias, int bias_type,
+                                        const void *offsets, int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out,
+                                        int precision, void *out, int out_type, void *stream);
+/* Its gradients, in `type`; each of d_x [n_rows][n_in], d_weight, d_bias may be NULL.  d_x at `precision`, the others as
+ * SCN_PRECISION_FP32. */
+SCN_API int scn_grouped_product_backward(const void *x, int64_t x_stride, int type, const void *weight, const void *d_out,
+                                         int64_t d_out_stride, const void *offsets, int offsets_64, int64_t n_rows, int n_groups,
+                                         int n_in, int n_out, int precision, void *d_x, void *d_weight, void *d_bias, void *stream);
+/* The same on 8-bit rows (scn_rms_norm_forward makes them): e4m3 q with scale [n_rows], e4m3 weight [n_groups][n_out][n_in]
+ * with weight_scale [n_groups][n_out]:  out[r][o] = scale[r] weight_scale[g][o] sum_i q[r][i] weight[g][o][i] + bias[g][o]. */
+SCN_API int scn_grouped_product_quantized(const void *q, int64_t q_stride, const float *scale, const void *weight,
+                                          const float *weight_scale, const void *bias, int bias_type, const void *offsets,
+                                          int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out, void *out, int out_type,
+                                          void *stream);
+/* Every wait inside the grouped products is bounded; one that ran out leaves a flag.  Waits for `stream`, reads and clears the
+ * current device's flag: SCN_ERR_CUDA if it was set.  scn_test_drop_barrier_arrival reaches the next
+ * scn_grouped_product_forward too. */
+SCN_API int scn_rows_poll_errors(void *stream);
+
 #ifdef __cplusplus
 }
 #endif

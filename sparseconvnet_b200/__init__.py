@@ -41,8 +41,9 @@ def Metadata(dim):
 
 from .layers import (InputLayer, OutputLayer, BLInputLayer, BLOutputLayer, SubmanifoldConvolution, ValidConvolution, Convolution,  # noqa: E402
                      Deconvolution, BatchNormalization, BatchNormReLU, BatchNormLeakyReLU, MaxPooling, AveragePooling, UnPooling,
-                     SparseToDense, NetworkInNetwork, RMSNormalization, AddRMSNormalization, Identity)
-from .rows import rms_norm, rms_norm_quantized  # noqa: E402
+                     SparseToDense, NetworkInNetwork, GroupedNetworkInNetwork, RMSNormalization, AddRMSNormalization, Identity)
+from .rows import (rms_norm, rms_norm_quantized, grouped_product, grouped_product_quantized,  # noqa: E402
+                   quantize_group_weights, poll_errors)
 from .containers import Sequential, ConcatTable, JoinTable, AddTable  # noqa: E402
 from .architectures import SparseVggNet, SparseResNet, UNet, FullyConvolutionalNet  # noqa: E402
 from .optim import AdamW, adamw_step  # noqa: E402

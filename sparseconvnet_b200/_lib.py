@@ -70,6 +70,13 @@ SIGNATURES = {
                                              C.c_double, _vp]),
     "scn_adamw_step": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_double, _vp, C.c_double,
                                  C.c_double, C.c_double, C.c_double, C.c_uint32, _vp]),
+    "scn_grouped_product_forward": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int, C.c_int64, C.c_int, C.c_int,
+                                              C.c_int, C.c_int, _vp, C.c_int, _vp]),
+    "scn_grouped_product_backward": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, C.c_int64, _vp, C.c_int, C.c_int64, C.c_int,
+                                               C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp]),
+    "scn_grouped_product_quantized": (C.c_int, [_vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_int, _vp, C.c_int, C.c_int64, C.c_int,
+                                                C.c_int, C.c_int, _vp, C.c_int, _vp]),
+    "scn_rows_poll_errors": (C.c_int, [_vp]),
     "scn_rms_norm_forward": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, C.c_int, _vp, C.c_int64, C.c_int, C.c_double, _vp, _vp,
                                        C.c_int, _vp, _vp, _vp]),
     "scn_rms_norm_backward": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, _vp, _vp,

@@ -1313,6 +1313,149 @@ SCN_FN(adamw_step) {
   SCN_END
 }
 
+// Offsets of groups of rows: int64 or int32 [groups + 1] on the rows' device
+struct Offsets {
+  at::Tensor t;
+  int wide, groups;
+  Offsets(PyObject *o, const at::Tensor &like) {
+    const at::Tensor &given = on_gpu(o, "offsets");
+    if (given.scalar_type() != at::kLong && given.scalar_type() != at::kInt) fail("offsets must be int64 or int32");
+    if (given.dim() != 1 || given.size(0) < 2) fail("offsets must have one entry more than there are groups");
+    if (given.device() != like.device()) fail("offsets are on another device than the rows");
+    t = given.contiguous();
+    wide = given.scalar_type() == at::kLong;
+    groups = (int)std::min<int64_t>(given.size(0) - 1, 1 << 30);
+  }
+};
+
+const at::Tensor &matrix(PyObject *o, const char *name) {
+  const at::Tensor &t = on_gpu(o, name);
+  if (t.dim() != 2) fail("%s must be a matrix", name);
+  return t;
+}
+
+struct GroupedProductNode : ag::Node {
+  ag::SavedVariable rows_, weight_, offsets_;
+  bool with_bias = false;
+  int precision = 0;
+  std::string name() const override { return "GroupedProductBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    rows_.reset_data();
+    weight_.reset_data();
+    offsets_.reset_data();
+  }
+  ag::variable_list apply(ag::variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ag::variable_list result(3);
+    if (!grads[0].defined()) return result;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_product: its gradient cannot be differentiated again (create_graph)");
+    const at::NoGradGuard no_grad;
+    const at::Tensor x = rows_.unpack(), w = weight_.unpack().contiguous(), offsets = offsets_.unpack();
+    // (a gradient of another type than the operands', as float32 results of 16-bit operands have, is rounded to theirs: the
+    // tensor core multiplies values of one type)
+    const at::Tensor dy = as_rows(grads[0].to(x.scalar_type()));
+    const OnDevice on(x);
+    const int64_t n = x.size(0), groups = w.size(0), nin = w.size(1), nout = w.size(2);
+    at::Tensor dx, dw, db;
+    if (task_should_compute_output(0)) dx = at::empty({n, nin}, x.options());
+    if (task_should_compute_output(1)) dw = at::empty(w.sizes(), w.options());
+    if (with_bias && task_should_compute_output(2)) db = at::empty({groups, nout}, w.options());
+    const int type = x.scalar_type() == at::kFloat ? SCN_TYPE_FLOAT32 : x.scalar_type() == at::kHalf ? SCN_TYPE_FLOAT16 : SCN_TYPE_BFLOAT16;
+    auto out = [](const at::Tensor &t) { return t.defined() ? raw(t) : nullptr; };
+    check_free(scn_grouped_product_backward(raw(x), row_stride(x), type, raw(w), raw(dy), row_stride(dy), raw(offsets),
+                                            offsets.scalar_type() == at::kLong, n, (int)groups, (int)nin, (int)nout, precision, out(dx),
+                                            out(dw), out(db), on.stream));
+    result[0] = dx, result[1] = dw, result[2] = db;
+    return result;
+  }
+};
+
+at::ScalarType scalar_type(int code) { return code == SCN_TYPE_FLOAT32 ? at::kFloat : code == SCN_TYPE_FLOAT16 ? at::kHalf : at::kBFloat16; }
+
+// (x [n, nIn], weight [groups, nIn, nOut], offsets, bias or None, scn_type of the result or -1, precision, precision of the
+//  input's gradient) -> [n, nOut]
+SCN_FN(grouped_product) {
+  SCN_BEGIN(7)
+  const at::Tensor &x = matrix(a[0], "x"), &weight = on_gpu(a[1], "weight");
+  const int type = type_of(x, "x");
+  const Offsets offsets(a[2], x);
+  int out_type = (int)PyLong_AsLong(a[4]);
+  const int precision = (int)PyLong_AsLong(a[5]), back = (int)PyLong_AsLong(a[6]);
+  if (PyErr_Occurred()) throw Fail{};
+  if (out_type < 0) out_type = type;
+  if (weight.dim() != 3 || weight.size(1) != x.size(1) || weight.size(0) != offsets.groups || weight.size(2) < 1 || x.size(1) < 1)
+    fail("weight must be [groups, nIn, nOut] with %lld groups and nIn = %lld", (long long)offsets.groups, (long long)x.size(1));
+  if (weight.scalar_type() != x.scalar_type() || weight.device() != x.device()) fail("weight must have the type and the device of x");
+  if (weight.size(1) > (1 << 20) || weight.size(2) > (1 << 20)) fail("too many planes");
+  at::Tensor bias;
+  if (a[3] != Py_None) {
+    bias = on_gpu(a[3], "bias");
+    if (bias.dim() != 2 || bias.size(0) != weight.size(0) || bias.size(1) != weight.size(2) || bias.scalar_type() != x.scalar_type() ||
+        bias.device() != x.device())
+      fail("bias must be [groups, nOut] with the type and the device of x");
+  }
+  no_tangents(x, weight, bias);
+  at::Tensor rows, out;
+  {
+    const at::NoGradGuard no_grad;
+    rows = as_rows(x);
+    const at::Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+    const OnDevice on(x);
+    out = at::empty({x.size(0), weight.size(2)}, x.options().dtype(scalar_type(out_type)));
+    SCN_CALL(scn_grouped_product_forward(raw(rows), row_stride(rows), type, raw(w), raw(b), type, raw(offsets.t), offsets.wide, x.size(0),
+                                         offsets.groups, (int)weight.size(1), (int)weight.size(2), precision, raw(out), out_type, on.stream));
+  }
+  if (ag::compute_requires_grad(x, weight, bias)) {
+    std::shared_ptr<GroupedProductNode> node(new GroupedProductNode(), ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(x, weight, bias));
+    node->rows_ = ag::SavedVariable(rows, false);
+    node->weight_ = ag::SavedVariable(weight, false);
+    node->offsets_ = ag::SavedVariable(offsets.t, false);
+    node->with_bias = bias.defined(), node->precision = back;
+    ag::set_history(out, node);
+  }
+  return THPVariable_Wrap(std::move(out));
+  SCN_END
+}
+
+// (q [n, nIn] e4m3, scale [n], weight [groups, nOut, nIn] e4m3, weight_scale [groups, nOut], offsets, bias or None, scn_type of
+//  the result) -> [n, nOut]
+SCN_FN(grouped_product_quantized) {
+  SCN_BEGIN(7)
+  const at::Tensor &q = matrix(a[0], "q"), &scale = on_gpu(a[1], "scale"), &weight = on_gpu(a[2], "weight"), &weight_scale = on_gpu(a[3], "weight_scale");
+  if (q.scalar_type() != at::kFloat8_e4m3fn || weight.scalar_type() != at::kFloat8_e4m3fn) fail("q and weight must be float8_e4m3fn");
+  if (scale.scalar_type() != at::kFloat || weight_scale.scalar_type() != at::kFloat) fail("scale and weight_scale must be float32");
+  const Offsets offsets(a[4], q);
+  const int out_type = (int)PyLong_AsLong(a[6]);
+  if (PyErr_Occurred()) throw Fail{};
+  const int64_t n = q.size(0), nin = q.size(1);
+  if (weight.dim() != 3 || weight.size(0) != offsets.groups || weight.size(2) != nin || weight.size(1) < 1 || nin < 1)
+    fail("weight must be [groups, nOut, nIn] with %lld groups and nIn = %lld", (long long)offsets.groups, (long long)nin);
+  const int64_t nout = weight.size(1);
+  if (nin > (1 << 20) || nout > (1 << 20)) fail("too many planes");
+  if (scale.dim() != 1 || scale.size(0) != n) fail("scale must have one entry per row");
+  if (weight_scale.dim() != 2 || weight_scale.size(0) != weight.size(0) || weight_scale.size(1) != nout) fail("weight_scale must be [groups, nOut]");
+  at::Tensor bias;
+  int bias_type = 0;
+  if (a[5] != Py_None) {
+    bias = on_gpu(a[5], "bias");
+    bias_type = type_of(bias, "bias");
+    if (bias.dim() != 2 || bias.size(0) != weight.size(0) || bias.size(1) != nout) fail("bias must be [groups, nOut]");
+  }
+  for (const at::Tensor *t : {&scale, &weight, &weight_scale, (const at::Tensor *)&bias})
+    if (t->defined() && t->device() != q.device()) fail("all operands must be on the rows' device");
+  if (ag::compute_requires_grad(scale, weight_scale, bias)) fail("a product of 8-bit rows has no gradient: call it under torch.no_grad()");
+  const at::NoGradGuard no_grad;
+  const at::Tensor rows = as_rows(q), s = scale.contiguous(), w = weight.contiguous(), ws = weight_scale.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+  const OnDevice on(q);
+  at::Tensor out = at::empty({n, nout}, s.options().dtype(scalar_type(out_type)));
+  SCN_CALL(scn_grouped_product_quantized(raw(rows), row_stride(rows), (const float *)raw(s), raw(w), (const float *)raw(ws), raw(b), bias_type,
+                                         raw(offsets.t), offsets.wide, n, offsets.groups, (int)nin, (int)nout, raw(out), out_type, on.stream));
+  return THPVariable_Wrap(std::move(out));
+  SCN_END
+}
+
 // (check function): how a failing status becomes an exception
 SCN_FN(set_check) {
   SCN_BEGIN(1)
@@ -1331,7 +1474,8 @@ PyMethodDef methods[] = {
     SCN_METHOD(active_sites),            SCN_METHOD(strided_size),       SCN_METHOD(transposed_size),
     SCN_METHOD(convolution_train),       SCN_METHOD(batchnorm_train),    SCN_METHOD(pooling_train),
     SCN_METHOD(strided_chain_start),     SCN_METHOD(rows_affine_train),       SCN_METHOD(input_layer),             SCN_METHOD(versions),           SCN_METHOD(set_check),
-    SCN_METHOD(rms_norm),                SCN_METHOD(adamw_step),         {nullptr, nullptr, 0, nullptr}};
+    SCN_METHOD(rms_norm),                SCN_METHOD(adamw_step),
+    SCN_METHOD(grouped_product),         SCN_METHOD(grouped_product_quantized),                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,878 @@
+// Products of ragged groups of rows, each with its group's own weights, on tcgen05 tensor cores.
+//
+//     forward        y[r]  = x[r] W[g] (+ b[g])       for offsets[g] <= r < offsets[g + 1]
+//     input          dx[r] = dy[r] W[g]^T
+//     weights        dW[g] = sum over the rows of g of x[r]^T dy[r]
+//     8 bits         y[r]  = s[r] S[g] (q[r] Q[g]) + b[g]        (e4m3 values, a scale per row and per group and output plane)
+//
+// The groups' sizes are known on the device only: every block sums the tiles of the groups before it looks for its own
+// (one scan at the start of the kernel), and takes every gridDim.x-th tile.  One kernel for all of them; what differs is
+// which planes of an operand lie next to each other in memory (K-major: those that are summed over, M- / N-major: the
+// others) and, for the weights' gradient, that a tile's sum runs over rows and has to end inside a stage: there the rows
+// of the next group are overwritten with zeros before the tensor core sees them (0 times what stands there could be NaN).
+//
+//   arithmetic  16-bit and 8-bit values as they are, fp32 sums.  fp32 values as bf16 parts (k_group_parts): x = h + m + l
+//               holds all 24 bits, and the products h h, h m, m h, h l, l h, m m leave out 2^-24 of a product; two parts and
+//               h h, h m, m h leave out 2^-17.  The tensor core cuts its running sum off at every instruction, half a unit
+//               of 2^-24 of it on average, so for fp32 results a sum is handed over to the registers of the epilogue warps
+//               every kDrain steps, and the products with an m or l have an accumulator of their own (they are 2^-8 as large).
+//   tile        128 x TN, TN = 256 for 16- and 8-bit values, 128 where parts or fp32 results take the second half of the
+//               tensor memory, 64 where wider tiles would leave SMs without work.  Two accumulators: one is read while the
+//               next tile is summed.
+//   roles       one warp copies tiles in (TMA, 128-byte swizzle, a ring over all of shared memory), one issues the
+//               instructions, eight read the accumulators, scale, add the bias, round and store.
+//   small groups  rows behind a group's last are not copied (boxes of 32 rows): their accumulator rows hold anything and are
+//               not stored.
+//
+// Every wait is bounded; what gave up is reported by scn_rows_poll_errors.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "rows.cuh"
+#include "tc_ptx.cuh"
+
+namespace scn {
+namespace {
+
+constexpr int kEpilogueWarps = 8, kThreads = (2 + kEpilogueWarps) * 32;
+constexpr int kTileM = 128, kRow = 128;      // bytes of an operand row in a stage
+constexpr int kStageRows = 64;               // rows (weights' gradient) or 16-bit values of K in a stage
+constexpr int kBoxRows = 32;                 // rows of a copy of the left operand
+constexpr int kRing = 196608;                // shared memory of the ring
+constexpr int kMostGroups = 1024;
+constexpr int kDrain = 4;                    // steps (of four instructions a product) between two hand-overs
+constexpr int kMostStages = 8;
+
+__device__ int g_flag;  // set by a kernel that gave up
+
+struct GroupParams {
+  const void *offsets;
+  int off64, groups;
+  int n_rows;
+  int k, n, m;             // rows: sum over k planes, n results; weights: m x n results, sum over rows
+  int n_tiles, m_tiles;    // m_tiles: weights only
+  int chunk;               // weights: rows of a unit
+  int stages;
+  unsigned idesc;          // without N
+  void *out;
+  int out_type, vectors;   // vectors: a row of results takes 16-byte stores
+  float *partial;          // weights: [unit of a group of several units][m][n]
+  const void *bias;
+  int bias_type;
+  const float *row_scale, *col_scale;
+  int drop;                // test: leave out the first arrival
+};
+
+struct Shared {
+  unsigned long long full[kMostStages], empty[kMostStages], ready[2], taken[2];
+  unsigned tmem;
+  int abort, issued;
+  int warp_sums[kThreads / 32];
+  int first[kMostGroups + 3];  // units (of rows) before the group
+  int begin[kMostGroups + 2], end[kMostGroups + 2];
+  int part[kMostGroups];       // weights: units before the group among the groups of several units, -1: one unit
+};
+
+// What a unit of work is
+struct Unit {
+  int group, row, rows, n0, m0;  // row: first row; rows: of the tile (rows) or of the sum (weights)
+  int part;                      // weights: the partial sum that this unit makes, -1: the gradient itself
+};
+
+__device__ __forceinline__ int offset_at(const GroupParams &P, int g) {
+  const long long v = P.off64 ? __ldg((const long long *)P.offsets + g) : (long long)__ldg((const int *)P.offsets + g);
+  return (int)min(max(v, 0ll), (long long)P.n_rows);
+}
+
+__device__ __forceinline__ int units_of(const GroupParams &P, bool weights, int rows) {
+  return weights ? max(1, (rows + P.chunk - 1) / P.chunk) : (rows + kTileM - 1) / kTileM;
+}
+
+// Sum (or maximum) of v >= 0 over the threads before this one
+template <bool MAX>
+__device__ __forceinline__ int over_before(int v, int *warp_sums) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int upto = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto = MAX ? max(upto, o) : upto + o;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  int before = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) before = 0;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) before = MAX ? max(before, warp_sums[w]) : before + warp_sums[w];
+  __syncthreads();
+  return before;
+}
+
+// Where the groups begin and end, and the units before each.  A group begins at the largest offset up to its own, so that
+// groups never overlap and their units fit what was made for them, whatever the offsets are.  Rows: groups G and G + 1 are
+// the rows behind and in front of all groups, whose results are zeros.
+template <bool WEIGHTS>
+__device__ __forceinline__ void scan_groups(const GroupParams &P, Shared &S) {
+  const int G = P.groups, tid = threadIdx.x, each = (G + 2 + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int from = tid * each, to = min(from + each, G + 1);
+  int most = 0;
+  for (int g = from; g < to; ++g) most = max(most, S.begin[g] = offset_at(P, g));
+  most = over_before<true>(most, S.warp_sums);
+  for (int g = from; g < to; ++g) S.begin[g] = most = max(most, S.begin[g]);
+  __syncthreads();
+  const int all = WEIGHTS ? G : G + 2, last = min(from + each, all);
+  int sum = 0, parts = 0;
+  for (int g = from; g < last; ++g) {
+    const int end = g < G ? S.begin[g + 1] : g == G ? P.n_rows : S.begin[0], begin = g <= G ? S.begin[g] : 0;
+    S.end[g] = end;
+    const int units = units_of(P, WEIGHTS, end - begin);
+    sum += units;
+    if (units > 1) parts += units;
+  }
+  int before = over_before<false>(sum, S.warp_sums), parts_before = WEIGHTS ? over_before<false>(parts, S.warp_sums) : 0;
+  for (int g = from; g < last; ++g) {
+    if (g > G) S.begin[g] = 0;
+    const int units = units_of(P, WEIGHTS, S.end[g] - S.begin[g]);
+    S.first[g] = before;
+    before += units;
+    if (WEIGHTS) {
+      S.part[g] = units > 1 ? parts_before : -1;
+      if (units > 1) parts_before += units;
+    }
+    if (g == all - 1) S.first[all] = before;
+  }
+  __syncthreads();
+}
+
+template <bool WEIGHTS, int TN>
+__device__ __forceinline__ Unit unit_at(const GroupParams &P, const Shared &S, long long u) {
+  const int all = WEIGHTS ? P.groups : P.groups + 2;
+  const int tiles = WEIGHTS ? P.n_tiles * P.m_tiles : P.n_tiles;
+  const int r = (int)(u / tiles), t = (int)(u - (long long)r * tiles);
+  int lo = 0, hi = all - 1;  // the last group that begins at or before r: groups without a unit share their start with the next
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (S.first[mid] <= r)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int each = WEIGHTS ? P.chunk : kTileM, row = S.begin[lo] + (r - S.first[lo]) * each;
+  return {lo, row, min(each, S.end[lo] - row), (WEIGHTS ? t % P.n_tiles : t) * TN, WEIGHTS ? t / P.n_tiles * kTileM : 0,
+          WEIGHTS && S.part[lo] >= 0 ? S.part[lo] + r - S.first[lo] : -1};
+}
+
+__device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w, unsigned long long *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <bool F8>
+__device__ __forceinline__ void mma_if(unsigned lead, unsigned d, unsigned a_lo, unsigned a_hi, unsigned b_lo, unsigned b_hi, unsigned idesc,
+                                       unsigned accumulate) {
+  if (!F8) {
+    mma_bf16_if(lead, d, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.u32 e, %7, 0;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+  }
+}
+
+// 128-byte swizzle; `next`: bytes to the operand's next 64 values along M or N (M- / N-major), not looked at otherwise
+__device__ __forceinline__ unsigned desc_lo(unsigned addr, unsigned next) { return ((addr >> 4) & 0x3FFF) | ((next >> 4) << 16); }
+constexpr unsigned kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+
+// The products of parts, largest first
+template <int P>
+struct Products {
+  static constexpr int N = P == 1 ? 1 : P == 2 ? 3 : 6;
+};
+__host__ __device__ constexpr int part_a(int i) { return i == 2 || i == 5 ? 1 : i == 4 ? 2 : 0; }  // hh hm mh hl lh mm
+__host__ __device__ constexpr int part_b(int i) { return i == 1 || i == 5 ? 1 : i == 3 ? 2 : 0; }
+
+__device__ __forceinline__ float value_at(const void *p, int type, long long i) {
+  return type == SCN_TYPE_FLOAT32 ? __ldg((const float *)p + i)
+         : type == SCN_TYPE_BFLOAT16 ? __bfloat162float(__ldg((const __nv_bfloat16 *)p + i))
+                                     : __half2float(__ldg((const __half *)p + i));
+}
+
+// 32 results of a row from column c on
+__device__ __forceinline__ void store32(void *out, int type, int vectors, long long at, int left, const float (&v)[32]) {
+  if (vectors && left >= 32) {
+    if (type == SCN_TYPE_FLOAT32) {
+      float4 *q = reinterpret_cast<float4 *>((float *)out + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+      uint4 *q = reinterpret_cast<uint4 *>((unsigned short *)out + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = type == SCN_TYPE_BFLOAT16 ? pair(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __nv_bfloat16())
+                                           : pair(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __half());
+        q[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (i >= left) break;
+    if (type == SCN_TYPE_FLOAT32)
+      ((float *)out)[at + i] = v[i];
+    else if (type == SCN_TYPE_BFLOAT16)
+      ((__nv_bfloat16 *)out)[at + i] = __float2bfloat16_rn(v[i]);
+    else
+      ((__half *)out)[at + i] = __float2half_rn(v[i]);
+  }
+}
+
+template <bool WEIGHTS, bool F8>
+__device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, int lane_row, int c, float (&v)[32]) {
+  if (WEIGHTS) {
+    if (u.m0 + lane_row >= P.m) return;
+    const bool part = u.part >= 0;
+    const long long row = (part ? (long long)u.part : u.group) * P.m + u.m0 + lane_row;
+    store32(part ? (void *)P.partial : P.out, part ? (int)SCN_TYPE_FLOAT32 : P.out_type, part ? P.n % 4 == 0 : P.vectors, row * P.n + c,
+            P.n - c, v);
+    return;
+  }
+  if (lane_row >= u.rows) return;
+  const bool real = u.group < P.groups;
+  if (F8 && real) {
+    const float s = __ldg(P.row_scale + u.row + lane_row);
+    const float *S = P.col_scale + (long long)u.group * P.n + c;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = c + i < P.n ? v[i] * s * __ldg(S + i) : 0.f;
+  }
+  if (P.bias && real) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < P.n) v[i] += value_at(P.bias, P.bias_type, (long long)u.group * P.n + c + i);
+  }
+  store32(P.out, P.out_type, P.vectors, (long long)(u.row + lane_row) * P.n + c, P.n - c, v);
+}
+
+template <int PARTS, int TN, bool SUMS, bool WEIGHTS, bool B_ROWS, bool F8>
+__global__ void __launch_bounds__(kThreads, 1)
+k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupParams P) {
+  SCN_GRID_WAIT();
+  constexpr int kABytes = kTileM * kRow, kBBytes = TN * kRow, kStage = PARTS * (kABytes + kBBytes), kStages = kRing / kStage;
+  static_assert(kStages <= kMostStages && kStages >= 2, "ring");
+  constexpr int kAccs = PARTS > 1 ? 2 : 1, kColumns = 256;  // tensor memory: two times 256 columns
+  static_assert(kAccs * TN <= kColumns, "accumulators");
+  extern __shared__ unsigned char raw[];
+  unsigned char *ring = raw + (1024 - smem_u32(raw) % 1024) % 1024;
+  __shared__ Shared S;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  volatile int *abort = &S.abort;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&S.full[i], 1), mbar_init(&S.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&S.ready[i], 1), mbar_init(&S.taken[i], kEpilogueWarps);
+    S.abort = 0;
+    S.issued = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(&S.tmem, 512);
+  scan_groups<WEIGHTS>(P, S);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = S.tmem;
+  const int all = WEIGHTS ? P.groups : P.groups + 2;
+  const long long units = (long long)S.first[all] * P.n_tiles * (WEIGHTS ? P.m_tiles : 1);
+  constexpr int kPerStage = F8 ? 2 * kStageRows : kStageRows;  // values of K in a stage
+  auto steps_of = [&](const Unit &u) { return WEIGHTS ? (u.rows + kStageRows - 1) / kStageRows : u.group < P.groups ? (P.k + kPerStage - 1) / kPerStage : 0; };
+
+  // ==== copies ====
+  if (warp == 0) {
+    const bool lead = elect_one();
+    int step = 0;
+    bool ok = true;
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const int steps = steps_of(u);
+      const int a_boxes = WEIGHTS ? 2 : (u.rows + kBoxRows - 1) / kBoxRows;
+      const unsigned bytes = PARTS * ((WEIGHTS ? kABytes : a_boxes * kBoxRows * kRow) + kBBytes);
+      for (int k = 0; k < steps; ++k, ++step) {
+        const int st = step % kStages;
+        if (step >= kStages && !mbar_wait_warp(&S.empty[st], (step / kStages - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        if (lead) {
+          const unsigned a = smem_u32(ring) + st * kStage, b = a + PARTS * kABytes;
+          mbar_expect_tx(&S.full[st], bytes);
+          for (int p = 0; p < PARTS; ++p) {
+            if (WEIGHTS) {
+              for (int j = 0; j < 2; ++j) load_tile(a + p * kABytes + j * kStageRows * kRow, &map_a, u.m0 + 64 * j, u.row + k * kStageRows, p, 0, &S.full[st]);
+              for (int j = 0; j < TN / 64; ++j) load_tile(b + p * kBBytes + j * kStageRows * kRow, &map_b, u.n0 + 64 * j, u.row + k * kStageRows, p, 0, &S.full[st]);
+            } else {
+              for (int j = 0; j < a_boxes; ++j) load_tile(a + p * kABytes + j * kBoxRows * kRow, &map_a, k * kPerStage, u.row + j * kBoxRows, p, 0, &S.full[st]);
+              if (B_ROWS)  // weights [k][n]: 64 values of n to a row
+                for (int j = 0; j < TN / 64; ++j) load_tile(b + p * kBBytes + j * kStageRows * kRow, &map_b, u.n0 + 64 * j, k * kStageRows, u.group, p, &S.full[st]);
+              else
+                load_tile(b + p * kBBytes, &map_b, k * kPerStage, u.n0, u.group, p, &S.full[st]);
+            }
+          }
+          S.issued = step + 1;
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== instructions ====
+  else if (warp == 1) {
+    const unsigned lead = elect_one();
+    int step = 0, turn = 0;
+    bool ok = true;
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const int steps = steps_of(u);
+      const unsigned idesc = P.idesc | (unsigned)(min(TN, (P.n - u.n0 + 15) / 16 * 16) >> 3) << 17;
+      for (int k = 0; k < steps; ++k, ++step) {
+        const bool begins = k == 0 || (SUMS && k % kDrain == 0), ends = k == steps - 1 || (SUMS && k % kDrain == kDrain - 1);
+        if (begins && turn >= 2 && !mbar_wait_warp(&S.taken[turn & 1], ((turn >> 1) - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        const int st = step % kStages;
+        if (!mbar_wait_warp(&S.full[st], (step / kStages) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        const unsigned a = smem_u32(ring) + st * kStage, b = a + PARTS * kABytes;
+        int instructions = 4;
+        if (WEIGHTS) {
+          const int left = u.rows - k * kStageRows;
+          if (left < kStageRows) {  // the rows behind the sum's last, up to a whole instruction: zeros
+            instructions = (left + 15) / 16;
+            const int gap = (instructions * 16 - left) * 8;  // 16-byte pieces of one 64 x 64 block
+            constexpr int kBlocks = PARTS * (2 + TN / 64);
+            for (int q = lane; q < gap * kBlocks; q += 32)
+              *reinterpret_cast<uint4 *>(ring + st * kStage + q / gap * (kStageRows * kRow) + left * kRow + q % gap * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        tc_fence_after();
+        const unsigned d = tmem + (turn & 1) * kColumns;
+        for (int j = 0; j < instructions; ++j) {
+#pragma unroll
+          for (int q = 0; q < Products<PARTS>::N; ++q) {
+            const unsigned pa = a + part_a(q) * kABytes + j * (WEIGHTS ? 16 * kRow : 32), pb = b + part_b(q) * kBBytes + j * (WEIGHTS || B_ROWS ? 16 * kRow : 32);
+            const unsigned fresh = begins && j == 0 && (q == 0 || q == 1);
+            mma_if<F8>(lead, d + (q ? TN : 0), desc_lo(pa, WEIGHTS ? kStageRows * kRow : 16), kDescHi, desc_lo(pb, WEIGHTS || B_ROWS ? kStageRows * kRow : 16),
+                       kDescHi, idesc, !fresh);
+          }
+        }
+        if (!(P.drop && blockIdx.x == 0 && step == 0)) tc_commit_if(lead, &S.empty[st]);
+        if (ends) {
+          tc_commit_if(lead, &S.ready[turn & 1]);
+          ++turn;
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== results ====
+  else {
+    const int quarter = warp % 4, half = (warp - 2) / 4;  // (a warp reaches the tensor memory's lanes 32 (warp % 4) on)
+    constexpr int kMine = TN / 2;
+    const int lane_row = quarter * 32 + lane;
+    int turn = 0;
+    bool ok = true;
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const int steps = steps_of(u), columns = min(P.n - u.n0 - half * kMine, kMine);
+      const int turns = steps == 0 ? 0 : SUMS ? (steps + kDrain - 1) / kDrain : 1;
+      float sum[SUMS ? kMine : 1];
+#pragma unroll
+      for (int c = 0; c < (SUMS ? kMine : 1); ++c) sum[c] = 0.f;
+      for (int t = 0; t < turns; ++t, ++turn) {
+        if (!mbar_wait_warp(&S.ready[turn & 1], (turn >> 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const unsigned from = tmem + ((unsigned)(quarter * 32) << 16) + (turn & 1) * kColumns + half * kMine;
+#pragma unroll
+        for (int c = 0; c < kMine; c += 32) {
+          if (c >= columns) break;
+          float v[32];
+          tmem_ld32(from + c, v);
+          if (SUMS) {
+            float low[32];
+            if (kAccs == 2) tmem_ld32(from + TN + c, low);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sum[SUMS ? c + e : 0] += kAccs == 2 ? v[e] + low[e] : v[e];
+          } else {
+            finish32<WEIGHTS, F8>(P, u, lane_row, u.n0 + half * kMine + c, v);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.taken[turn & 1]);
+      }
+      if (!ok) break;
+      if (SUMS || turns == 0) {
+#pragma unroll
+        for (int c = 0; c < kMine; c += 32) {
+          if (c >= columns) break;
+          float v[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = SUMS ? sum[SUMS ? c + e : 0] : 0.f;
+          finish32<WEIGHTS, F8>(P, u, lane_row, u.n0 + half * kMine + c, v);
+        }
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (S.abort) {  // what is under way into this block's memory lands before the block ends
+    if (tid == 0) {
+      atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+      for (int s = 0; s < kStages; ++s)
+        if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
+    }
+  }
+  __syncwarp();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Rows of a matrix as `parts` matrices of 16-bit values (or 8-bit ones, copied), planes padded with zeros to whole 16 bytes:
+// what the copies above need where the operand is fp32 or its rows do not lie on 16 bytes.  One thread per 16 bytes of
+// a part.  Bound by HBM: 4 bytes in, 2 per part out.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256)
+k_group_parts(const T *__restrict__ src, long long stride, int planes, long long n_pieces, int per_row, long long part_bytes,
+              unsigned char *__restrict__ dst) {
+  SCN_GRID_WAIT();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n_pieces) return;
+  constexpr int N = sizeof(T) == 1 ? 16 : 8;
+  const long long row = i / per_row;
+  const int c = (int)(i - row * per_row) * N;
+  const T *from = src + row * stride + c;
+  unsigned w[3][4] = {};
+  if (sizeof(T) == 4) {
+    float v[8];
+    if (c + 8 <= planes && ((uintptr_t)from & 15) == 0) {
+      const float4 p = __ldg((const float4 *)from), q = __ldg((const float4 *)from + 1);
+      v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < planes ? __ldg((const float *)from + j) : 0.f;
+    }
+    unsigned short h[3][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float rest = v[j];
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+        // (a value above bf16's largest is cut off instead; an infinity or a NaN has no further parts)
+        if (PARTS > 1 && (b & 0x7FFF) == 0x7F80 && isfinite(rest)) b = __float_as_uint(rest) >> 16;
+        h[p][j] = (unsigned short)b;
+        rest = isfinite(rest) ? rest - __uint_as_float(b << 16) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[p][j] = h[p][2 * j] | (unsigned)h[p][2 * j + 1] << 16;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const unsigned v = c + j < planes ? (sizeof(T) == 2 ? (unsigned)__ldg((const unsigned short *)from + j) : (unsigned)__ldg((const unsigned char *)from + j)) : 0u;
+      w[0][j * (int)sizeof(T) / 4] |= v << (j * (int)sizeof(T) % 4 * 8);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4 *>(dst + p * part_bytes + i * 16) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+__device__ __forceinline__ void put_value(void *out, int type, long long at, float v) {
+  if (type == SCN_TYPE_FLOAT32)
+    ((float *)out)[at] = v;
+  else if (type == SCN_TYPE_BFLOAT16)
+    ((__nv_bfloat16 *)out)[at] = __float2bfloat16_rn(v);
+  else
+    ((__half *)out)[at] = __float2half_rn(v);
+}
+
+// The gradients of the groups of several units: their partial sums, in order
+__global__ void __launch_bounds__(256)
+k_group_sum(const __grid_constant__ GroupParams P) {
+  SCN_GRID_WAIT();
+  __shared__ Shared S;
+  scan_groups<true>(P, S);
+  const long long size = (long long)P.m * P.n;
+  for (int g = 0; g < P.groups; ++g) {
+    if (S.part[g] < 0) continue;
+    const int units = S.first[g + 1] - S.first[g];
+    const float *from = P.partial + S.part[g] * size;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long long)gridDim.x * 256) {
+      float v = 0.f;
+      for (int u = 0; u < units; ++u) v += __ldg(from + u * size + i);
+      put_value(P.out, P.out_type, g * size + i, v);
+    }
+  }
+}
+
+// db[g] = sum of a group's rows: a block takes a unit of P.chunk rows and 32 planes, 8 rows at a time (m = 1)
+__global__ void __launch_bounds__(256)
+k_group_bias(const __grid_constant__ GroupParams P, const void *d_out, long long stride, int type) {
+  SCN_GRID_WAIT();
+  __shared__ Shared S;
+  __shared__ float part[8][33];
+  scan_groups<true>(P, S);
+  const int lane = threadIdx.x % 32, along = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+  for (long long u = blockIdx.y; u < S.first[P.groups]; u += gridDim.y) {
+    const Unit unit = unit_at<true, 64>(P, S, u);
+    float v = 0.f;
+    if (c < P.n) {
+      int r = along;
+      for (; r + 24 < unit.rows; r += 32) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = value_at(d_out, type, (long long)(unit.row + r + 8 * j) * stride + c);
+        v += (x[0] + x[1]) + (x[2] + x[3]);
+      }
+      for (; r < unit.rows; r += 8) v += value_at(d_out, type, (long long)(unit.row + r) * stride + c);
+    }
+    part[along][lane] = v;
+    __syncthreads();
+    if (along == 0 && c < P.n) {
+#pragma unroll
+      for (int j = 1; j < 8; ++j) v += part[j][lane];
+      if (unit.part >= 0)
+        P.partial[(long long)unit.part * P.n + c] = v;
+      else
+        put_value(P.out, P.out_type, (long long)unit.group * P.n + c, v);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int encoder(EncodeTiled *out) {  // looked up through the runtime: the library loads on a machine without a driver
+  static std::atomic<EncodeTiled> known{nullptr};
+  *out = known.load();
+  if (!*out) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    SCN_CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
+    SCN_REQUIRE(fn && found == cudaDriverEntryPointSuccess, SCN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    known.store(*out = (EncodeTiled)fn);
+  }
+  return SCN_OK;
+}
+
+// An operand as the tensor maps need it
+struct Operand {
+  const void *p = nullptr;
+  int bytes = 2;             // of a value
+  long long stride = 0;      // bytes from row to row
+  long long matrix = 0;      // bytes from group to group (weights)
+  long long part = 0;        // bytes from part to part
+};
+
+int make_map(CUtensorMap *map, const Operand &o, int type, long long planes, long long rows, long long groups, int parts, int box_planes, int box_rows) {
+  EncodeTiled encode;
+  SCN_TRY(encoder(&encode));
+  const long long matrix = o.matrix ? o.matrix : rows * o.stride, part = o.part ? o.part : groups * matrix;
+  const cuuint64_t dims[4] = {(cuuint64_t)planes, (cuuint64_t)rows, (cuuint64_t)groups, (cuuint64_t)parts};
+  const cuuint64_t strides[3] = {(cuuint64_t)o.stride, (cuuint64_t)matrix, (cuuint64_t)part};
+  const cuuint32_t box[4] = {(cuuint32_t)box_planes, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = type == SCN_TYPE_E4M3     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : type == SCN_TYPE_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = encode(map, t, 4, const_cast<void *>(o.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  SCN_REQUIRE(r == CUDA_SUCCESS, SCN_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return SCN_OK;
+}
+
+// The operand where it lies, or a copy in parts
+int operand(const void *p, long long stride, int planes, long long rows, int type, int parts, Scratch &scratch, cudaStream_t stream, Operand *o) {
+  const int size = type == SCN_TYPE_FLOAT32 ? 4 : type == SCN_TYPE_E4M3 ? 1 : 2;
+  if (type != SCN_TYPE_FLOAT32 && (uintptr_t)p % 16 == 0 && stride * size % 16 == 0 && stride > 0 && stride * size < (1ll << 40)) {
+    *o = Operand{p, size, stride * size, 0, 0};
+    return SCN_OK;
+  }
+  const int held = size == 1 ? 1 : 2, per_row = (int)ceil_div((long long)planes * held, 16);
+  const long long row_bytes = per_row * 16ll, part_bytes = rows * row_bytes, pieces = rows * per_row;
+  unsigned char *to = nullptr;
+  SCN_TRY(scratch.get(&to, (size_t)(parts * part_bytes)));
+  const unsigned blocks = (unsigned)ceil_div(pieces, 256);
+#define SCN_PARTS(T, N) SCN_LAUNCH((k_group_parts<T, N>), blocks, 256, 0, stream, (const T *)p, stride, planes, pieces, per_row, part_bytes, to)
+  if (type == SCN_TYPE_FLOAT32) {
+    if (parts == 3)
+      SCN_PARTS(float, 3);
+    else if (parts == 2)
+      SCN_PARTS(float, 2);
+    else
+      SCN_PARTS(float, 1);
+  } else if (size == 2) {
+    SCN_PARTS(unsigned short, 1);
+  } else {
+    SCN_PARTS(unsigned char, 1);
+  }
+#undef SCN_PARTS
+  SCN_CUDA_CHECK(cudaGetLastError());
+  *o = Operand{to, held, row_bytes, 0, part_bytes};
+  return SCN_OK;
+}
+
+constexpr int kSms = 148;
+
+template <int PARTS, int TN, bool SUMS, bool WEIGHTS, bool B_ROWS, bool F8>
+int launch(const CUtensorMap &a, const CUtensorMap &b, GroupParams P, long long most_units, cudaStream_t stream) {
+  constexpr size_t smem = kRing + 1024;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  SCN_CUDA_CHECK(cudaGetDevice(&dev));
+  SCN_REQUIRE(dev >= 0 && dev < 64, SCN_ERR_UNSUPPORTED, "device index %d unsupported", dev);
+  constexpr auto kernel = k_group_product<PARTS, TN, SUMS, WEIGHTS, B_ROWS, F8>;
+  if (!configured[dev].load()) {
+    SCN_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured[dev].store(true);
+  }
+  int blocks = 0;
+  SCN_TRY(resident_blocks<kernel>(kThreads, smem, &blocks));
+  SCN_LAUNCH(kernel, (unsigned)std::min<long long>(blocks, most_units), kThreads, smem, stream, a, b, P);
+  SCN_CUDA_CHECK(cudaGetLastError());
+  return SCN_OK;
+}
+
+// Columns of a tile: as wide as the results are, but no wider than leaves every SM a tile.
+int tile_columns(long long row_tiles, int n, int most) {
+  int tn = most;
+  while (tn > 64 && (n <= tn / 2 || row_tiles * ceil_div(n, tn) < kSms)) tn /= 2;
+  return tn;
+}
+
+unsigned idesc_of(int type, bool a_rows, bool b_rows) {  // fp32 sums, M = 128; types: bf16 1, f16 0, e4m3 0
+  const unsigned t = type == SCN_TYPE_FLOAT16 || type == SCN_TYPE_E4M3 ? 0 : 1;
+  return (1u << 4) | (t << 7) | (t << 10) | ((unsigned)a_rows << 15) | ((unsigned)b_rows << 16) | ((unsigned)(kTileM >> 4) << 24);
+}
+
+struct Groups {
+  const void *offsets;
+  int off64;
+  long long n_rows;
+  int groups;
+};
+
+// y = x W: `b_rows`: the weights' n lie next to each other ([k][n]), else their k ([n][k])
+int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_rows, int parts, int type, int k, int n, void *out, int out_type,
+                 const void *bias, int bias_type, const float *row_scale, const float *col_scale, int drop, cudaStream_t stream) {
+  const bool f8 = type == SCN_TYPE_E4M3, sums = !f8 && (parts > 1 || out_type == SCN_TYPE_FLOAT32);
+  const long long row_tiles = G.n_rows / kTileM + std::min<long long>(G.groups + 2, G.n_rows);
+  const int tn = tile_columns(row_tiles, n, sums ? 128 : 256);
+  GroupParams P{};
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
+  P.idesc = idesc_of(type, false, b_rows);
+  const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
+  P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
+  P.bias = bias, P.bias_type = bias_type, P.row_scale = row_scale, P.col_scale = col_scale, P.drop = drop;
+  const int per = f8 ? 128 : 64;
+  CUtensorMap a, b;
+  SCN_TRY(make_map(&a, x, type, k, G.n_rows, parts, 1, per, kBoxRows));  // (parts lie where groups would)
+  SCN_TRY(b_rows ? make_map(&b, w, type, n, k, G.groups, parts, 64, 64) : make_map(&b, w, type, k, n, G.groups, parts, per, tn));
+  const long long most = row_tiles * P.n_tiles;
+#define SCN_TN(PARTS, SUMS, B_ROWS, F8)                                                                       \
+  (tn == 64 ? launch<PARTS, 64, SUMS, false, B_ROWS, F8>(a, b, P, most, stream)                               \
+   : tn == 128 ? launch<PARTS, 128, SUMS, false, B_ROWS, F8>(a, b, P, most, stream)                           \
+               : launch<PARTS, SUMS ? 128 : 256, SUMS, false, B_ROWS, F8>(a, b, P, most, stream))
+#define SCN_MAJOR(PARTS, SUMS) (b_rows ? SCN_TN(PARTS, SUMS, true, false) : SCN_TN(PARTS, SUMS, false, false))
+  if (f8) return SCN_TN(1, false, false, true);
+  if (!sums) return SCN_MAJOR(1, false);
+  return parts == 1 ? SCN_MAJOR(1, true) : parts == 2 ? SCN_MAJOR(2, true) : SCN_MAJOR(3, true);
+#undef SCN_MAJOR
+#undef SCN_TN
+}
+
+// Rows of a unit of a sum over rows, such that a group that has all of them still gives every SM some: twice as many units as
+// SMs with `tiles` tiles of the result to a unit.
+int chunk_of(long long n_rows, long long tiles) {
+  const long long wanted = std::max<long long>(1, 2 * kSms / tiles);
+  return (int)std::max<long long>(512, ceil_div(ceil_div(n_rows, wanted), 64) * 64);
+}
+
+int sum_parts(GroupParams P, cudaStream_t stream) {
+  const long long size = (long long)P.m * P.n;
+  SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(ceil_div(size, 256), 4 * kSms), 256, 0, stream, P);
+  SCN_CUDA_CHECK(cudaGetLastError());
+  return SCN_OK;
+}
+
+// dW = x^T dy by groups
+int weights_product(const Groups &G, const Operand &x, const Operand &dy, int parts, int type, int m, int n, void *out, int out_type,
+                    Scratch &scratch, cudaStream_t stream) {
+  const long long m_tiles = ceil_div(m, kTileM);
+  const int tn = tile_columns(m_tiles * std::max<long long>(G.groups, G.n_rows / 512), n, parts > 1 ? 128 : 256);
+  GroupParams P{};
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.m = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
+  P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
+  P.idesc = idesc_of(type, true, true);
+  const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
+  P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
+  const bool split = G.n_rows > P.chunk;
+  // (a group of several units has more than P.chunk rows: at most n_rows / chunk of them, with one unit more each than that)
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * m * n));
+  CUtensorMap a, b;
+  SCN_TRY(make_map(&a, x, type, m, G.n_rows, parts, 1, 64, kStageRows));
+  SCN_TRY(make_map(&b, dy, type, n, G.n_rows, parts, 1, 64, kStageRows));
+  const long long most = (ceil_div(G.n_rows, P.chunk) + G.groups) * P.m_tiles * P.n_tiles;
+#define SCN_TN(PARTS, SUMS)                                                                 \
+  (tn == 64 ? launch<PARTS, 64, SUMS, true, true, false>(a, b, P, most, stream)             \
+   : tn == 128 ? launch<PARTS, 128, SUMS, true, true, false>(a, b, P, most, stream)         \
+               : launch<PARTS, SUMS ? 128 : 256, SUMS, true, true, false>(a, b, P, most, stream))
+  SCN_TRY(parts == 1 ? SCN_TN(1, false) : SCN_TN(3, true));
+#undef SCN_TN
+  return split ? sum_parts(P, stream) : SCN_OK;
+}
+
+int bias_sums(const Groups &G, const void *dy, long long stride, int type, int n, void *out, int out_type, Scratch &scratch, cudaStream_t stream) {
+  GroupParams P{};
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.m = 1, P.n = n, P.m_tiles = P.n_tiles = 1;
+  P.chunk = chunk_of(G.n_rows, std::max<long long>(1, ceil_div(n, 32) / 4));
+  P.out = out, P.out_type = out_type;
+  const bool split = G.n_rows > P.chunk;
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * n));
+  const long long units = ceil_div(G.n_rows, P.chunk) + G.groups;
+  SCN_LAUNCH(k_group_bias, dim3((unsigned)ceil_div(n, 32), (unsigned)std::min<long long>(units, 1024)), 256, 0, stream, P, dy, stride, type);
+  SCN_CUDA_CHECK(cudaGetLastError());
+  return split ? sum_parts(P, stream) : SCN_OK;
+}
+
+int parts_of(int type, int precision) {
+  return type != SCN_TYPE_FLOAT32 ? 1 : precision == SCN_PRECISION_FP32 ? 3 : precision == SCN_PRECISION_BF16 ? 1 : 2;
+}
+bool is_type(int t) { return t == SCN_TYPE_FLOAT32 || t == SCN_TYPE_BFLOAT16 || t == SCN_TYPE_FLOAT16; }
+
+int check_sizes(const void *offsets, int64_t n_rows, int n_groups, int n_in, int n_out) {
+  SCN_REQUIRE(n_rows >= 0 && n_in >= 1 && n_out >= 1, SCN_ERR_BAD_ARG, "grouped_product: bad sizes");
+  SCN_REQUIRE(n_groups >= 1 && n_groups <= kMostGroups, SCN_ERR_UNSUPPORTED, "grouped_product: 1 to %d groups", kMostGroups);
+  SCN_REQUIRE(n_rows < (1ll << 31) - 65536, SCN_ERR_UNSUPPORTED, "grouped_product: too many rows");
+  SCN_REQUIRE(n_in <= (1 << 20) && n_out <= (1 << 20), SCN_ERR_UNSUPPORTED, "grouped_product: too many planes");
+  SCN_REQUIRE(n_rows == 0 || offsets, SCN_ERR_BAD_ARG, "grouped_product: null argument");
+  return SCN_OK;
+}
+
+}  // namespace
+
+extern thread_local int g_drop_arrival;  // test hook (conv_tc.cu)
+
+}  // namespace scn
+
+using namespace scn;
+
+extern "C" {
+
+int scn_grouped_product_forward(const void *x, int64_t x_stride, int type, const void *weight, const void *bias, int bias_type,
+                                const void *offsets, int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out, int precision,
+                                void *out, int out_type, void *stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  SCN_REQUIRE(is_type(type) && is_type(out_type) && (!bias || is_type(bias_type)), SCN_ERR_BAD_ARG, "grouped_product: unknown type");
+  SCN_REQUIRE(precision >= SCN_PRECISION_FP32 && precision <= SCN_PRECISION_TF32X3, SCN_ERR_BAD_ARG, "grouped_product: unknown precision");
+  SCN_TRY(check_sizes(offsets, n_rows, n_groups, n_in, n_out));
+  if (n_rows == 0) return SCN_OK;
+  SCN_REQUIRE(x && weight && out, SCN_ERR_BAD_ARG, "grouped_product: null argument");
+  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  const int parts = parts_of(type, precision), held = type == SCN_TYPE_FLOAT32 ? SCN_TYPE_BFLOAT16 : type;
+  Scratch scratch(stream);
+  Operand a, b;
+  SCN_TRY(operand(x, x_stride, n_in, n_rows, type, parts, scratch, stream, &a));
+  SCN_TRY(operand(weight, n_out, n_out, (long long)n_groups * n_in, type, parts, scratch, stream, &b));
+  b.matrix = b.stride * n_in;
+  const int drop = g_drop_arrival;
+  g_drop_arrival = 0;
+  return rows_product(G, a, b, true, parts, held, n_in, n_out, out, out_type, bias, bias_type, nullptr, nullptr, drop, stream);
+}
+
+int scn_grouped_product_backward(const void *x, int64_t x_stride, int type, const void *weight, const void *d_out, int64_t d_out_stride,
+                                 const void *offsets, int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out, int precision,
+                                 void *d_x, void *d_weight, void *d_bias, void *stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  SCN_REQUIRE(is_type(type), SCN_ERR_BAD_ARG, "grouped_product: unknown type");
+  SCN_REQUIRE(precision >= SCN_PRECISION_FP32 && precision <= SCN_PRECISION_TF32X3, SCN_ERR_BAD_ARG, "grouped_product: unknown precision");
+  SCN_TRY(check_sizes(offsets, n_rows, n_groups, n_in, n_out));
+  if (n_rows == 0) {
+    const size_t size = type == SCN_TYPE_FLOAT32 ? 4 : 2;
+    if (d_weight) SCN_CUDA_CHECK(cudaMemsetAsync(d_weight, 0, size * n_groups * n_in * n_out, stream));
+    if (d_bias) SCN_CUDA_CHECK(cudaMemsetAsync(d_bias, 0, size * n_groups * n_out, stream));
+    return SCN_OK;
+  }
+  SCN_REQUIRE(d_out && (!d_x || weight) && (!d_weight || x), SCN_ERR_BAD_ARG, "grouped_product: null argument");
+  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  const int held = type == SCN_TYPE_FLOAT32 ? SCN_TYPE_BFLOAT16 : type;
+  // the input's gradient at the precision asked for, the weights' always as fp32
+  const int dx_parts = parts_of(type, precision), dw_parts = parts_of(type, SCN_PRECISION_FP32);
+  Scratch scratch(stream);
+  Operand dy;
+  if (d_x || d_weight) SCN_TRY(operand(d_out, d_out_stride, n_out, n_rows, type, d_weight ? dw_parts : dx_parts, scratch, stream, &dy));
+  if (d_x) {
+    Operand w;
+    SCN_TRY(operand(weight, n_out, n_out, (long long)n_groups * n_in, type, dx_parts, scratch, stream, &w));
+    w.matrix = w.stride * n_in;
+    SCN_TRY(rows_product(G, dy, w, false, dx_parts, held, n_out, n_in, d_x, type, nullptr, 0, nullptr, nullptr, 0, stream));
+  }
+  if (d_weight) {
+    Operand a;
+    SCN_TRY(operand(x, x_stride, n_in, n_rows, type, dw_parts, scratch, stream, &a));
+    SCN_TRY(weights_product(G, a, dy, dw_parts, held, n_in, n_out, d_weight, type, scratch, stream));
+  }
+  return d_bias ? bias_sums(G, d_out, d_out_stride, type, n_out, d_bias, type, scratch, stream) : SCN_OK;
+}
+
+int scn_grouped_product_quantized(const void *q, int64_t q_stride, const float *scale, const void *weight, const float *weight_scale,
+                                  const void *bias, int bias_type, const void *offsets, int offsets_64, int64_t n_rows, int n_groups,
+                                  int n_in, int n_out, void *out, int out_type, void *stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  SCN_REQUIRE(is_type(out_type) && (!bias || is_type(bias_type)), SCN_ERR_BAD_ARG, "grouped_product: unknown type");
+  SCN_TRY(check_sizes(offsets, n_rows, n_groups, n_in, n_out));
+  if (n_rows == 0) return SCN_OK;
+  SCN_REQUIRE(q && scale && weight && weight_scale && out, SCN_ERR_BAD_ARG, "grouped_product: null argument");
+  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  Scratch scratch(stream);
+  Operand a, b;
+  SCN_TRY(operand(q, q_stride, n_in, n_rows, SCN_TYPE_E4M3, 1, scratch, stream, &a));
+  SCN_TRY(operand(weight, n_in, n_in, (long long)n_groups * n_out, SCN_TYPE_E4M3, 1, scratch, stream, &b));
+  b.matrix = b.stride * n_out;
+  return rows_product(G, a, b, false, 1, SCN_TYPE_E4M3, n_in, n_out, out, out_type, bias, bias_type, scale, weight_scale, 0, stream);
+}
+
+int scn_rows_poll_errors(void *stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  int *at = nullptr, flag = 0;
+  SCN_CUDA_CHECK(cudaGetSymbolAddress((void **)&at, g_flag));
+  SCN_CUDA_CHECK(cudaMemcpyAsync(&flag, at, sizeof(int), cudaMemcpyDeviceToHost, stream));
+  note_host_wait();
+  SCN_CUDA_CHECK(cudaStreamSynchronize(stream));
+  if (!flag) return SCN_OK;
+  SCN_CUDA_CHECK(cudaMemsetAsync(at, 0, sizeof(int), stream));
+  SCN_REQUIRE(false, SCN_ERR_CUDA, "a wait inside a grouped product ran out: its results are incomplete");
+}
+
+}  // extern "C"

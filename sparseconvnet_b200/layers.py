@@ -697,6 +697,37 @@ class NetworkInNetwork(Module):
         return "NetworkInNetwork%d->%d" % (self.nIn, self.nOut)
 
 
+class GroupedNetworkInNetwork(Module):
+    """A NetworkInNetwork with weights of their own for every group of rows: sources, samples or experts; weight [nGroups, nIn,
+    nOut].  Takes ``[tensor, offsets]``: the rows from offsets[g] up to offsets[g + 1] (int64 or int32, on the GPU) are
+    group g, rows of no group become zeros.  Not in the reference."""
+
+    def __init__(self, nGroups, nIn, nOut, bias):
+        Module.__init__(self)
+        self.nGroups = nGroups
+        self.nIn = nIn
+        self.nOut = nOut
+        self.weight = Parameter(torch.empty(nGroups, nIn, nOut).normal_(0, (2.0 / nIn) ** 0.5))
+        if bias:
+            self.bias = Parameter(torch.zeros(nGroups, nOut))
+
+    def forward(self, input):
+        input, offsets = input
+        assert input.features.nelement() == 0 or input.features.size(1) == self.nIn
+        output = SparseConvNetTensor(metadata=input.metadata, spatial_size=input.spatial_size)
+        features = input.features if input.features.dim() == 2 else input.features.new_zeros(0, self.nIn)
+        output.features = rows.grouped_product(features, parameter(self, "weight"), offsets, parameter(self, "bias"))
+        SCN.flop_counter.add(float(input.features.size(0) * self.nIn * self.nOut))
+        _pkg.forward_pass_hidden_states += output.features.nelement()
+        return output
+
+    def input_spatial_size(self, out_size):
+        return out_size
+
+    def __repr__(self):
+        return "GroupedNetworkInNetwork%dx%d->%d" % (self.nGroups, self.nIn, self.nOut)
+
+
 class Identity(Module):
     def forward(self, input):
         return input

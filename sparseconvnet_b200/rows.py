@@ -38,3 +38,45 @@ def rms_norm_quantized(x, weight=None, residual=None, eps=1e-6):
     tensor of the shape of x, scale float32 of its leading sizes: q * scale is the norm, and the largest value of a row is
     448 in q (a row of zeros is zeros).  No gradient."""
     return SCN._binding.rms_norm(x, _row_weight(weight), residual, eps, _E4M3)
+
+
+def grouped_product(x, weight, offsets, bias=None, out_dtype=None):
+    """Every group of rows times its own weights: for offsets[g] <= r < offsets[g + 1]
+
+        out[r] = x[r] @ weight[g] (+ bias[g])
+
+    x: [n, nIn], rows in group order; weight: [groups, nIn, nOut]; bias: [groups, nOut]; all of one type.  offsets: int64 or
+    int32 CUDA tensor [groups + 1], not decreasing (1 to 1024 groups, empty ones among them); the host never waits for
+    them.  Rows of no group (before the first, behind the last) are zeros and have no gradient.
+    bfloat16 and float16 are multiplied as they are; float32 by ``set_precision``: 'fp32' with all bits, 'tf32x3' and 'tf32'
+    to 2^-17 of a product, 'bf16' rounded to bfloat16 (the input's gradient by ``set_backward_precision``, the weights'
+    with all bits).  Sums are float32, results ``out_dtype`` (None: the type of x).  A float32 row with an infinity may
+    give NaN.  Differentiable (once) in x, weight and bias."""
+    return SCN._binding.grouped_product(x, weight, offsets, bias, _type_code(out_dtype, "out_dtype"), SCN._precision,
+                                        SCN._backward_precision)
+
+
+def quantize_group_weights(weight):
+    """Weights [groups, nIn, nOut] as ``grouped_product_quantized`` reads them: (float8_e4m3fn [groups, nOut, nIn], float32
+    scales [groups, nOut]), the largest value of a column at 448.  Done once for a network that serves."""
+    w = weight.detach().float().transpose(1, 2)
+    scale = w.abs().amax(2).clamp_min(1e-30) / 448
+    return (w / scale[:, :, None]).contiguous().to(torch.float8_e4m3fn), scale
+
+
+def grouped_product_quantized(q, scale, weight, weight_scale, offsets, bias=None, out_dtype=torch.bfloat16):
+    """``grouped_product`` on 8-bit rows, as ``rms_norm_quantized`` makes them, and 8-bit weights
+    (``quantize_group_weights``):
+
+        out[r, o] = scale[r] * weight_scale[g, o] * sum_i q[r, i] weight[g, o, i] (+ bias[g, o])
+
+    The products are exact and summed in float32; no gradient."""
+    if out_dtype not in _TYPES:
+        raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
+    return SCN._binding.grouped_product_quantized(q, scale, weight, weight_scale, offsets, bias, _TYPES[out_dtype])
+
+
+def poll_errors():
+    """Waits for the current stream and raises if a wait inside a grouped product ran out since the last call (its results are
+    incomplete then).  The counterpart of ``Metadata.poll_errors``."""
+    SCN.check(SCN.lib.scn_rows_poll_errors(SCN._stream()))
