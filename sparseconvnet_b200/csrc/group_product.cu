@@ -54,6 +54,7 @@ struct GroupParams {
   int k, n, m;             // rows: sum over k planes, n results; weights: m x n results, sum over rows
   int n_tiles, m_tiles;    // m_tiles: weights only
   int chunk;               // weights: rows of a unit
+  int tile;                // rows of a unit (rows) or of a tile of the result (weights)
   int stages;
   unsigned idesc;          // without N
   void *out;
@@ -70,6 +71,7 @@ struct Shared {
   unsigned tmem;
   int abort, issued;
   int warp_sums[kThreads / 32];
+  __align__(16) float columns[kEpilogueWarps][32];
   int first[kMostGroups + 3];  // units (of rows) before the group
   int begin[kMostGroups + 2], end[kMostGroups + 2];
   int part[kMostGroups];       // weights: units before the group among the groups of several units, -1: one unit
@@ -87,7 +89,7 @@ __device__ __forceinline__ int offset_at(const GroupParams &P, int g) {
 }
 
 __device__ __forceinline__ int units_of(const GroupParams &P, bool weights, int rows) {
-  return weights ? max(1, (rows + P.chunk - 1) / P.chunk) : (rows + kTileM - 1) / kTileM;
+  return weights ? max(1, (rows + P.chunk - 1) / P.chunk) : (rows + P.tile - 1) / P.tile;
 }
 
 // Sum (or maximum) of v >= 0 over the threads before this one
@@ -158,8 +160,8 @@ __device__ __forceinline__ Unit unit_at(const GroupParams &P, const Shared &S, l
     else
       hi = mid - 1;
   }
-  const int each = WEIGHTS ? P.chunk : kTileM, row = S.begin[lo] + (r - S.first[lo]) * each;
-  return {lo, row, min(each, S.end[lo] - row), (WEIGHTS ? t % P.n_tiles : t) * TN, WEIGHTS ? t / P.n_tiles * kTileM : 0,
+  const int each = WEIGHTS ? P.chunk : P.tile, row = S.begin[lo] + (r - S.first[lo]) * each;
+  return {lo, row, min(each, S.end[lo] - row), (WEIGHTS ? t % P.n_tiles : t) * TN, WEIGHTS ? t / P.n_tiles * P.tile : 0,
           WEIGHTS && S.part[lo] >= 0 ? S.part[lo] + r - S.first[lo] : -1};
 }
 
@@ -235,8 +237,52 @@ __device__ __forceinline__ void store32(void *out, int type, int vectors, long l
   }
 }
 
-template <bool WEIGHTS, bool F8>
-__device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, int lane_row, int c, float (&v)[32]) {
+// What belongs to a unit's columns and rows, read by a warp of the epilogue while the unit is still being summed: lane l has
+// columns l, l + 32 ..
+template <int COLS, bool WEIGHTS, bool F8>
+struct Terms {
+  float bias[COLS / 32], scale[F8 ? COLS / 32 : 1], row_scale;
+  bool with_bias, real;
+  __device__ __forceinline__ void read(const GroupParams &P, const Unit &u, int c0, int lane_row, int lane) {
+    real = !WEIGHTS && u.group < P.groups;
+    with_bias = real && P.bias;
+    row_scale = F8 && real && lane_row < u.rows ? __ldg(P.row_scale + u.row + lane_row) : 0.f;
+#pragma unroll
+    for (int j = 0; j < COLS / 32; ++j) {
+      const int c = c0 + 32 * j + lane;
+      const bool in = real && c < P.n;
+      bias[j] = with_bias && in ? value_at(P.bias, P.bias_type, (long long)u.group * P.n + c) : 0.f;
+      if (F8) scale[F8 ? j : 0] = in ? __ldg(P.col_scale + (long long)u.group * P.n + c) : 0.f;
+    }
+  }
+};
+
+// 32 results of the row `lane_row` of a unit, from column c = c0 + 32 j on; the whole warp comes here.  `shared`: 32 floats of the
+// warp, through which every lane sees all columns' terms.
+template <int COLS, bool WEIGHTS, bool F8>
+__device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, const Terms<COLS, WEIGHTS, F8> &terms, int j, int lane_row, int c,
+                                         float *shared, float (&v)[32]) {
+  const int lane = threadIdx.x % 32;
+  if (F8 && terms.real) {
+    shared[lane] = terms.scale[F8 ? j : 0];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 s = reinterpret_cast<const float4 *>(shared)[i];
+      v[4 * i] *= s.x * terms.row_scale, v[4 * i + 1] *= s.y * terms.row_scale, v[4 * i + 2] *= s.z * terms.row_scale, v[4 * i + 3] *= s.w * terms.row_scale;
+    }
+    __syncwarp();
+  }
+  if (!WEIGHTS && terms.with_bias) {
+    shared[lane] = terms.bias[j];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = reinterpret_cast<const float4 *>(shared)[i];
+      v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
+    }
+    __syncwarp();
+  }
   if (WEIGHTS) {
     if (u.m0 + lane_row >= P.m) return;
     const bool part = u.part >= 0;
@@ -245,20 +291,7 @@ __device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, in
             P.n - c, v);
     return;
   }
-  if (lane_row >= u.rows) return;
-  const bool real = u.group < P.groups;
-  if (F8 && real) {
-    const float s = __ldg(P.row_scale + u.row + lane_row);
-    const float *S = P.col_scale + (long long)u.group * P.n + c;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = c + i < P.n ? v[i] * s * __ldg(S + i) : 0.f;
-  }
-  if (P.bias && real) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (c + i < P.n) v[i] += value_at(P.bias, P.bias_type, (long long)u.group * P.n + c + i);
-  }
-  store32(P.out, P.out_type, P.vectors, (long long)(u.row + lane_row) * P.n + c, P.n - c, v);
+  if (lane_row < u.rows) store32(P.out, P.out_type, P.vectors, (long long)(u.row + lane_row) * P.n + c, P.n - c, v);
 }
 
 template <int PARTS, int TN, bool SUMS, bool WEIGHTS, bool B_ROWS, bool F8>
@@ -396,6 +429,8 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
       const int steps = steps_of(u), columns = min(P.n - u.n0 - half * kMine, kMine);
       const int turns = steps == 0 ? 0 : SUMS ? (steps + kDrain - 1) / kDrain : 1;
+      Terms<kMine, WEIGHTS, F8> terms;
+      terms.read(P, u, u.n0 + half * kMine, lane_row, lane);
       float sum[SUMS ? kMine : 1];
 #pragma unroll
       for (int c = 0; c < (SUMS ? kMine : 1); ++c) sum[c] = 0.f;
@@ -417,7 +452,7 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
             for (int e = 0; e < 32; ++e) sum[SUMS ? c + e : 0] += kAccs == 2 ? v[e] + low[e] : v[e];
           } else {
-            finish32<WEIGHTS, F8>(P, u, lane_row, u.n0 + half * kMine + c, v);
+            finish32(P, u, terms, c / 32, lane_row, u.n0 + half * kMine + c, S.columns[warp - 2], v);
           }
         }
         tc_fence_before();
@@ -432,7 +467,7 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = SUMS ? sum[SUMS ? c + e : 0] : 0.f;
-          finish32<WEIGHTS, F8>(P, u, lane_row, u.n0 + half * kMine + c, v);
+          finish32(P, u, terms, c / 32, lane_row, u.n0 + half * kMine + c, S.columns[warp - 2], v);
         }
       }
     }
@@ -520,13 +555,21 @@ k_group_sum(const __grid_constant__ GroupParams P) {
   __shared__ Shared S;
   scan_groups<true>(P, S);
   const long long size = (long long)P.m * P.n;
-  for (int g = 0; g < P.groups; ++g) {
+  for (int g = blockIdx.y; g < P.groups; g += gridDim.y) {
     if (S.part[g] < 0) continue;
     const int units = S.first[g + 1] - S.first[g];
     const float *from = P.partial + S.part[g] * size;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long long)gridDim.x * 256) {
       float v = 0.f;
-      for (int u = 0; u < units; ++u) v += __ldg(from + u * size + i);
+      int u = 0;
+      for (; u + 8 <= units; u += 8) {  // (added in order, asked for at once)
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __ldg(from + (u + j) * size + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v += x[j];
+      }
+      for (; u < units; ++u) v += __ldg(from + u * size + i);
       put_value(P.out, P.out_type, g * size + i, v);
     }
   }
@@ -603,8 +646,17 @@ int make_map(CUtensorMap *map, const Operand &o, int type, long long planes, lon
   const CUtensorMapDataType t = type == SCN_TYPE_E4M3     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                 : type == SCN_TYPE_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUresult r = encode(map, t, 4, const_cast<void *>(o.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto make = [&] {
+    return encode(map, t, 4, const_cast<void *>(o.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = make();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has not launched anything yet (autograd's): the driver wants its context bound
+    int dev = 0;
+    SCN_CUDA_CHECK(cudaGetDevice(&dev));
+    SCN_CUDA_CHECK(cudaSetDevice(dev));
+    r = make();
+  }
   SCN_REQUIRE(r == CUDA_SUCCESS, SCN_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
   return SCN_OK;
 }
@@ -688,6 +740,7 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
   const int tn = tile_columns(row_tiles, n, sums ? 128 : 256);
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.tile = kTileM;
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(type, false, b_rows);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
@@ -719,7 +772,8 @@ int chunk_of(long long n_rows, long long tiles) {
 
 int sum_parts(GroupParams P, cudaStream_t stream) {
   const long long size = (long long)P.m * P.n;
-  SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(ceil_div(size, 256), 4 * kSms), 256, 0, stream, P);
+  const long long across = std::min<long long>(ceil_div(size, 256), 4 * kSms), groups = std::min<long long>(P.groups, ceil_div(8 * kSms, across));
+  SCN_LAUNCH(k_group_sum, dim3((unsigned)across, (unsigned)groups), 256, 0, stream, P);
   SCN_CUDA_CHECK(cudaGetLastError());
   return SCN_OK;
 }
@@ -731,6 +785,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   const int tn = tile_columns(m_tiles * std::max<long long>(G.groups, G.n_rows / 512), n, parts > 1 ? 128 : 256);
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.tile = kTileM;
   P.m = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
   P.idesc = idesc_of(type, true, true);

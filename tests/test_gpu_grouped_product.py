@@ -294,6 +294,28 @@ def test_two_streams_at_once(cuda):
     assert all(torch.equal(g, want[k]) for k in range(2) for g in got[k])
 
 
+def test_a_thread_of_its_own(cuda):
+    """The call may be the first that a thread makes of the GPU, as in autograd's threads."""
+    import threading
+    o = offsets_of([30, 34])
+    x, w, dy = normal(64, 64, t=torch.bfloat16, seed=1).requires_grad_(), normal(2, 64, 64, t=torch.bfloat16, seed=2).requires_grad_(), normal(64, 64, t=torch.bfloat16, seed=3)
+    want = scn.grouped_product(x, w, o)
+    grads = torch.autograd.grad(want, [x, w], dy)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        with torch.no_grad():
+            got.append(scn.grouped_product(x, w, o))
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 3 and all(torch.equal(g, want) for g in got) and grads[0].shape == x.shape
+
+
 def test_refusals(cuda):
     x, w, o = normal(4, 8), normal(2, 8, 16), offsets_of([1, 3])
     for args, said in (((x, w[:1], o), "groups"), ((x, w, o[:1]), "offsets"), ((x, w.half(), o), "type"), ((x, w, o.float()), "int64 or int32"), ((x, w, o.cpu()), "CUDA"),
