@@ -68,8 +68,10 @@ struct GroupParams {
 
 struct Shared {
   unsigned long long full[kMostStages], empty[kMostStages], ready[2], taken[2];
+  unsigned long long tail[kMostStages], zeroed[kMostStages];  // pairs
   unsigned tmem;
   int abort, issued;
+  unsigned tails, tail_last;  // stages that have been a sum's end, and the parity of the last time
   int warp_sums[kThreads / 32];
   __align__(16) float columns[kEpilogueWarps][32];
   int first[kMostGroups + 3];  // units (of rows) before the group
@@ -487,6 +489,275 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
+// ---- pairs of blocks ------------------------------------------------------------------------------------------------------
+// The same products with two SMs on a tile of 256 x 256 (tcgen05 cta_group::2): each has 128 rows of the left operand, half of
+// the right one's columns and the accumulators of its 128 rows, and one of them issues for both.  A block then copies 32 KB
+// for what takes 48 KB alone.  That is what bounds wide layers: one block per tile drew 57 bytes per cycle and SM out of L2
+// (13.5 TB/s) at 61% of the tensor cores' time.
+// The leader's barriers count both blocks' copies and readings; its commits arrive in both blocks.
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned in_block(const void *p, unsigned rank) {  // the peer's (or own) shared memory
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_at(unsigned cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// mbar_wait_warp for barriers that the other block arrives at
+__device__ __forceinline__ bool wait_pair(unsigned long long *bar, unsigned parity, const volatile int *abort) {
+  const unsigned addr = smem_u32(bar);
+  for (unsigned it = 0; it < kWaitLimit; ++it) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    if (__any_sync(0xffffffffu, *abort != 0)) return false;
+  }
+  return false;
+}
+// into this block, counted by a barrier of either
+__device__ __forceinline__ void load_tile_pair(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w, unsigned cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(cluster_bar)
+      : "memory");
+}
+template <bool F8>
+__device__ __forceinline__ void mma_pair_if(unsigned lead, unsigned d, unsigned a_lo, unsigned a_hi, unsigned b_lo, unsigned b_hi, unsigned idesc,
+                                            unsigned accumulate) {
+  if (!F8)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.u32 e, %7, 0;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.u32 e, %7, 0;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair_if(unsigned lead, unsigned long long *bar) {  // arrives at `bar` of both blocks
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead), "h"((unsigned short)3)
+      : "memory");
+}
+
+constexpr int kPairN = 256;  // columns of a pair's tile
+
+template <bool WEIGHTS, bool B_ROWS, bool F8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupParams P) {
+  SCN_GRID_WAIT();
+  constexpr int kABytes = kTileM * kRow, kBBytes = kPairN / 2 * kRow, kStage = kABytes + kBBytes, kStages = kRing / kStage, kColumns = 256;
+  static_assert(kStages <= kMostStages, "ring");
+  extern __shared__ unsigned char raw[];
+  unsigned char *ring = raw + (1024 - smem_u32(raw) % 1024) % 1024;  // (at the same address in both blocks)
+  __shared__ Shared S;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const unsigned rank = cluster_rank();
+  volatile int *abort = &S.abort;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&S.full[i], 1), mbar_init(&S.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&S.ready[i], 1), mbar_init(&S.taken[i], 2 * kEpilogueWarps);
+    for (int i = 0; i < kStages; ++i) mbar_init(&S.tail[i], 1), mbar_init(&S.zeroed[i], 2);
+    S.abort = 0;
+    S.issued = 0;
+    S.tails = S.tail_last = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  scan_groups<WEIGHTS>(P, S);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // (barriers of both blocks exist)
+  tc_fence_after();
+  const unsigned tmem = S.tmem;
+  const int all = WEIGHTS ? P.groups : P.groups + 2;
+  const long long units = (long long)S.first[all] * P.n_tiles * (WEIGHTS ? P.m_tiles : 1);
+  const long long pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  constexpr int kPerStage = F8 ? 2 * kStageRows : kStageRows;
+  auto steps_of = [&](const Unit &u) { return WEIGHTS ? (u.rows + kStageRows - 1) / kStageRows : u.group < P.groups ? (P.k + kPerStage - 1) / kPerStage : 0; };
+  auto width_of = [&](const Unit &u) { return min(kPairN, (P.n - u.n0 + 31) / 32 * 32); };  // columns of the instruction
+  auto boxes_of = [&](const Unit &u, int r) { return WEIGHTS ? 2 : max(0, min(kTileM, u.rows - r * kTileM) + kBoxRows - 1) / kBoxRows; };
+
+  // ==== copies ====
+  if (warp == 0) {
+    const bool lead = elect_one();
+    int step = 0;
+    unsigned tails = 0;  // a bit per stage, the other way round after each sum that ended there
+    bool ok = true;
+    for (long long i = pair; i < units && ok; i += pairs) {
+      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const int steps = steps_of(u), n0 = u.n0 + (int)rank * (width_of(u) / 2), boxes = boxes_of(u, rank);
+      constexpr unsigned kBox = WEIGHTS ? kStageRows * kRow : kBoxRows * kRow;
+      const unsigned mine = boxes * kBox + kBBytes, both = (boxes_of(u, 0) + boxes_of(u, 1)) * kBox + 2 * kBBytes;
+      for (int k = 0; k < steps; ++k, ++step) {
+        const int st = step % kStages;
+        if (step >= kStages && !wait_pair(&S.empty[st], (step / kStages - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        // a sum that ends inside a stage: each block sees its own copies land, to overwrite what lies behind the last row
+        const bool tail = WEIGHTS && (k + 1) * kStageRows > u.rows;
+        if (lead) {
+          const unsigned a = smem_u32(ring) + st * kStage, b = a + kABytes, bar = tail ? in_block(&S.tail[st], rank) : in_block(&S.full[st], 0);
+          if (tail) {
+            mbar_expect_tx(&S.tail[st], mine);
+            if (rank == 0) mbar_arrive(&S.full[st]);
+            S.tails |= 1u << st, S.tail_last = (S.tail_last & ~(1u << st)) | (tails & (1u << st));
+          } else if (rank == 0) {
+            mbar_expect_tx(&S.full[st], both);
+          }
+          if (WEIGHTS) {
+            for (int j = 0; j < 2; ++j) load_tile_pair(a + j * kStageRows * kRow, &map_a, u.m0 + (int)rank * kTileM + 64 * j, u.row + k * kStageRows, 0, 0, bar);
+            for (int j = 0; j < 2; ++j) load_tile_pair(b + j * kStageRows * kRow, &map_b, n0 + 64 * j, u.row + k * kStageRows, 0, 0, bar);
+          } else {
+            for (int j = 0; j < boxes; ++j) load_tile_pair(a + j * kBoxRows * kRow, &map_a, k * kPerStage, u.row + (int)rank * kTileM + j * kBoxRows, 0, 0, bar);
+            if (B_ROWS)
+              for (int j = 0; j < 2; ++j) load_tile_pair(b + j * kStageRows * kRow, &map_b, n0 + 64 * j, k * kStageRows, u.group, 0, bar);
+            else
+              load_tile_pair(b, &map_b, k * kPerStage, n0, u.group, 0, bar);
+          }
+          S.issued = step + 1;
+        }
+        if (tail) tails ^= 1u << st;
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== instructions ====
+  else if (warp == 1) {
+    const unsigned lead = elect_one();
+    int step = 0, turn = 0;
+    unsigned tails = 0;
+    bool ok = true;
+    for (long long i = pair; i < units && ok; i += pairs) {
+      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const int steps = steps_of(u);
+      const unsigned idesc = P.idesc | (unsigned)(width_of(u) >> 3) << 17;
+      const int behind = WEIGHTS ? u.rows % kStageRows : 0;
+      if (rank == 0 && steps && turn >= 2 && !wait_pair(&S.taken[turn & 1], ((turn >> 1) - 1) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      for (int k = 0; k < steps; ++k, ++step) {
+        const int st = step % kStages;
+        int instructions = 4;
+        if (WEIGHTS && behind && k == steps - 1) {
+          instructions = (behind + 15) / 16;
+          if (!wait_pair(&S.tail[st], tails >> st & 1, abort)) {
+            ok = false;
+            break;
+          }
+          const int gap = (instructions * 16 - behind) * 8;
+          for (int q = lane; q < gap * 4; q += 32)
+            *reinterpret_cast<uint4 *>(ring + st * kStage + q / gap * (kStageRows * kRow) + behind * kRow + q % gap * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_at(in_block(&S.zeroed[st], 0));
+          if (rank == 0 && !wait_pair(&S.zeroed[st], tails >> st & 1, abort)) {
+            ok = false;
+            break;
+          }
+          tails ^= 1u << st;
+        }
+        if (rank != 0) continue;
+        if (!wait_pair(&S.full[st], (step / kStages) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const unsigned a = smem_u32(ring) + st * kStage, b = a + kABytes, d = tmem + (turn & 1) * kColumns;
+        for (int j = 0; j < instructions; ++j) {
+          const unsigned pa = a + j * (WEIGHTS ? 16 * kRow : 32), pb = b + j * (WEIGHTS || B_ROWS ? 16 * kRow : 32);
+          mma_pair_if<F8>(lead, d, desc_lo(pa, WEIGHTS ? kStageRows * kRow : 16), kDescHi, desc_lo(pb, WEIGHTS || B_ROWS ? kStageRows * kRow : 16), kDescHi,
+                          idesc, k > 0 || j > 0);
+        }
+        if (!(P.drop && blockIdx.x == 0 && step == 0)) commit_pair_if(lead, &S.empty[st]);
+        if (k == steps - 1) commit_pair_if(lead, &S.ready[turn & 1]);
+        __syncwarp();
+      }
+      turn += steps > 0;
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== results ====
+  else {
+    const int quarter = warp % 4, half = (warp - 2) / 4;
+    constexpr int kMine = kPairN / 2;
+    const int lane_row = (int)rank * kTileM + quarter * 32 + lane;
+    int turn = 0;
+    bool ok = true;
+    for (long long i = pair; i < units && ok; i += pairs) {
+      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const int columns = min(P.n - u.n0 - half * kMine, kMine);
+      const bool summed = steps_of(u) > 0;
+      Terms<kMine, WEIGHTS, F8> terms;
+      terms.read(P, u, u.n0 + half * kMine, lane_row, lane);
+      if (summed && !wait_pair(&S.ready[turn & 1], (turn >> 1) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const unsigned from = tmem + ((unsigned)(quarter * 32) << 16) + (turn & 1) * kColumns + half * kMine;
+#pragma unroll
+      for (int c = 0; c < kMine; c += 32) {
+        if (c >= columns) break;
+        float v[32];
+        if (summed) {
+          tmem_ld32(from + c, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        }
+        finish32(P, u, terms, c / 32, lane_row, u.n0 + half * kMine + c, S.columns[warp - 2], v);
+      }
+      if (summed) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(in_block(&S.taken[turn & 1], 0));
+        ++turn;
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (S.abort) {  // own copies land before the block ends; those of full steps are counted by the leader
+    if (tid == 0) {
+      atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+      if (rank == 0)
+        for (int s = 0; s < kStages; ++s)
+          if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
+      for (int s = 0; s < kStages; ++s)
+        if (S.tails >> s & 1) mbar_wait(&S.tail[s], S.tail_last >> s & 1);
+    }
+  }
+  __syncthreads();
+  cluster_sync();  // (nothing of the other block is under way into this one's barriers or out of its operands)
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
 // Rows of a matrix as `parts` matrices of 16-bit values (or 8-bit ones, copied), planes padded with zeros to whole 16 bytes:
 // what the copies above need where the operand is fp32 or its rows do not lie on 16 bytes.  One thread per 16 bytes of
 // a part.  Bound by HBM: 4 bytes in, 2 per part out.
@@ -713,6 +984,46 @@ int launch(const CUtensorMap &a, const CUtensorMap &b, GroupParams P, long long 
   return SCN_OK;
 }
 
+// Two blocks to a tile.  Worth it where the copies bound a tile: many rows to a group (a group ends in the middle of 256 rows
+// instead of 128 on average) and tiles enough for all pairs.
+bool paired(long long row_tiles_256, long long groups, int n) { return n > 128 && row_tiles_256 >= 2 * groups && row_tiles_256 * ceil_div(n, kPairN) >= kSms / 2; }
+
+template <bool WEIGHTS, bool B_ROWS, bool F8>
+int launch_pair(const CUtensorMap &a, const CUtensorMap &b, const GroupParams &P, long long most_units, cudaStream_t stream) {
+  constexpr size_t smem = kRing + 1024;
+  static std::atomic<int> known[64];  // pairs that the device holds at once
+  int dev = 0;
+  SCN_CUDA_CHECK(cudaGetDevice(&dev));
+  SCN_REQUIRE(dev >= 0 && dev < 64, SCN_ERR_UNSUPPORTED, "device index %d unsupported", dev);
+  constexpr auto kernel = k_group_pair<WEIGHTS, B_ROWS, F8>;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.blockDim = kThreads;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attr;
+  int pairs = known[dev].load();
+  if (!pairs) {
+    SCN_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    config.gridDim = 2;
+    config.attrs = attr + 1;
+    config.numAttrs = 1;
+    SCN_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&pairs, kernel, &config));
+    SCN_REQUIRE(pairs > 0, SCN_ERR_CUDA, "no pair of blocks fits the device");
+    known[dev].store(pairs);
+    config.attrs = attr;
+  }
+  config.numAttrs = 1;  // (the cluster's size is the kernel's own)
+  config.gridDim = (unsigned)(2 * std::min<long long>(pairs, most_units));
+  note_launch();
+  SCN_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, b, P));
+  return SCN_OK;
+}
+
 // Columns of a tile: as wide as the results are, but no wider than leaves every SM a tile.
 int tile_columns(long long row_tiles, int n, int most) {
   int tn = most;
@@ -720,9 +1031,9 @@ int tile_columns(long long row_tiles, int n, int most) {
   return tn;
 }
 
-unsigned idesc_of(int type, bool a_rows, bool b_rows) {  // fp32 sums, M = 128; types: bf16 1, f16 0, e4m3 0
+unsigned idesc_of(int type, bool a_rows, bool b_rows, int m) {  // fp32 sums; types: bf16 1, f16 0, e4m3 0
   const unsigned t = type == SCN_TYPE_FLOAT16 || type == SCN_TYPE_E4M3 ? 0 : 1;
-  return (1u << 4) | (t << 7) | (t << 10) | ((unsigned)a_rows << 15) | ((unsigned)b_rows << 16) | ((unsigned)(kTileM >> 4) << 24);
+  return (1u << 4) | (t << 7) | (t << 10) | ((unsigned)a_rows << 15) | ((unsigned)b_rows << 16) | ((unsigned)(m >> 4) << 24);
 }
 
 struct Groups {
@@ -737,20 +1048,25 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
                  const void *bias, int bias_type, const float *row_scale, const float *col_scale, int drop, cudaStream_t stream) {
   const bool f8 = type == SCN_TYPE_E4M3, sums = !f8 && (parts > 1 || out_type == SCN_TYPE_FLOAT32);
   const long long row_tiles = G.n_rows / kTileM + std::min<long long>(G.groups + 2, G.n_rows);
-  const int tn = tile_columns(row_tiles, n, sums ? 128 : 256);
+  const long long pair_tiles = G.n_rows / (2 * kTileM) + std::min<long long>(G.groups + 2, G.n_rows);
+  const bool pair = !sums && paired(pair_tiles, G.groups, n);
+  const int tn = pair ? kPairN : tile_columns(row_tiles, n, sums ? 128 : 256);
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
-  P.tile = kTileM;
+  P.tile = pair ? 2 * kTileM : kTileM;
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
-  P.idesc = idesc_of(type, false, b_rows);
+  P.idesc = idesc_of(type, false, b_rows, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
   P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
   P.bias = bias, P.bias_type = bias_type, P.row_scale = row_scale, P.col_scale = col_scale, P.drop = drop;
   const int per = f8 ? 128 : 64;
   CUtensorMap a, b;
   SCN_TRY(make_map(&a, x, type, k, G.n_rows, parts, 1, per, kBoxRows));  // (parts lie where groups would)
-  SCN_TRY(b_rows ? make_map(&b, w, type, n, k, G.groups, parts, 64, 64) : make_map(&b, w, type, k, n, G.groups, parts, per, tn));
-  const long long most = row_tiles * P.n_tiles;
+  SCN_TRY(b_rows ? make_map(&b, w, type, n, k, G.groups, parts, 64, 64) : make_map(&b, w, type, k, n, G.groups, parts, per, pair ? tn / 2 : tn));
+  const long long most = (pair ? pair_tiles : row_tiles) * P.n_tiles;
+  if (pair)
+    return f8 ? launch_pair<false, false, true>(a, b, P, most, stream)
+           : b_rows ? launch_pair<false, true, false>(a, b, P, most, stream) : launch_pair<false, false, false>(a, b, P, most, stream);
 #define SCN_TN(PARTS, SUMS, B_ROWS, F8)                                                                       \
   (tn == 64 ? launch<PARTS, 64, SUMS, false, B_ROWS, F8>(a, b, P, most, stream)                               \
    : tn == 128 ? launch<PARTS, 128, SUMS, false, B_ROWS, F8>(a, b, P, most, stream)                           \
@@ -763,10 +1079,10 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
 #undef SCN_TN
 }
 
-// Rows of a unit of a sum over rows, such that a group that has all of them still gives every SM some: twice as many units as
-// SMs with `tiles` tiles of the result to a unit.
+// Rows of a unit of a sum over rows, such that a group that has all of them still gives most SMs some: where there are fewer
+// than half as many tiles of the result as SMs, twice as many units as SMs.
 int chunk_of(long long n_rows, long long tiles) {
-  const long long wanted = std::max<long long>(1, 2 * kSms / tiles);
+  const long long wanted = tiles * 2 >= kSms ? 1 : 2 * kSms / tiles;
   return (int)std::max<long long>(512, ceil_div(ceil_div(n_rows, wanted), 64) * 64);
 }
 
@@ -781,14 +1097,17 @@ int sum_parts(GroupParams P, cudaStream_t stream) {
 // dW = x^T dy by groups
 int weights_product(const Groups &G, const Operand &x, const Operand &dy, int parts, int type, int m, int n, void *out, int out_type,
                     Scratch &scratch, cudaStream_t stream) {
-  const long long m_tiles = ceil_div(m, kTileM);
-  const int tn = tile_columns(m_tiles * std::max<long long>(G.groups, G.n_rows / 512), n, parts > 1 ? 128 : 256);
+  // (pairs: tiles of 256 x 256 of the result; a sum that ends inside a stage costs a pair 2 us, so not for sums of a few rows)
+  const bool pair = parts == 1 && m > kTileM && n > 128 && G.n_rows >= 256ll * G.groups &&
+                    ceil_div(m, 2 * kTileM) * ceil_div(n, kPairN) * std::max<long long>(G.groups, G.n_rows / 512) >= kSms / 2;
+  const long long m_tiles = ceil_div(m, pair ? 2 * kTileM : kTileM);
+  const int tn = pair ? kPairN : tile_columns(m_tiles * std::max<long long>(G.groups, G.n_rows / 512), n, parts > 1 ? 128 : 256);
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
-  P.tile = kTileM;
+  P.tile = pair ? 2 * kTileM : kTileM;
   P.m = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
-  P.idesc = idesc_of(type, true, true);
+  P.idesc = idesc_of(type, true, true, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
   P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
   const bool split = G.n_rows > P.chunk;
@@ -802,7 +1121,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   (tn == 64 ? launch<PARTS, 64, SUMS, true, true, false>(a, b, P, most, stream)             \
    : tn == 128 ? launch<PARTS, 128, SUMS, true, true, false>(a, b, P, most, stream)         \
                : launch<PARTS, SUMS ? 128 : 256, SUMS, true, true, false>(a, b, P, most, stream))
-  SCN_TRY(parts == 1 ? SCN_TN(1, false) : SCN_TN(3, true));
+  SCN_TRY((pair ? launch_pair<true, true, false>(a, b, P, most, stream) : parts == 1 ? SCN_TN(1, false) : SCN_TN(3, true)));
 #undef SCN_TN
   return split ? sum_parts(P, stream) : SCN_OK;
 }

@@ -61,7 +61,10 @@ def offsets_of(sizes, before=0, wide=True):
 SHAPES = [([1], 0, 0, 1, 1), ([1, 0, 2], 0, 0, 16, 16), ([5], 3, 2, 8, 24), ([128, 128], 0, 0, 64, 64), ([129, 0, 127, 1], 0, 5, 64, 96),
           ([33, 64, 0, 0, 200], 7, 0, 72, 136), ([300, 1, 17], 0, 0, 20, 3), ([40, 41], 0, 1, 3, 20), ([700, 90], 1, 1, 130, 257),
           ([64] * 9, 0, 0, 128, 320), ([1000, 2500, 37], 0, 0, 256, 128), ([20, 31], 0, 0, 1024, 512), ([0, 0], 4, 9, 32, 32),
-          ([3] * 100, 0, 0, 48, 40), ([4000], 0, 0, 40, 64)]
+          ([3] * 100, 0, 0, 48, 40), ([4000], 0, 0, 40, 64),
+          # tiles of two blocks: groups that end in the first and in the second block's rows, inside and at the end of a stage
+          ([3000, 0, 5000, 2900], 5, 3, 264, 300), ([2560, 2816, 4096, 1024], 0, 0, 512, 256), ([10001, 77, 1, 640], 0, 0, 136, 1000),
+          ([9000, 130], 1, 1, 1000, 264)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -336,16 +339,17 @@ def test_refusals(cuda):
 def test_a_wait_that_runs_out_is_reported(cuda):
     """Leaves out one arrival in one block: the call gives up in bounded time, poll_errors says so, the next call is right."""
     from sparseconvnet_b200._lib import lib
-    o = offsets_of([256])
-    x, w = normal(256, 4096, t=torch.bfloat16, seed=1), normal(1, 4096, 256, t=torch.bfloat16, seed=2)
-    want = scn.grouped_product(x, w, o)
-    scn.poll_errors()
-    lib.scn_test_drop_barrier_arrival()
-    scn.grouped_product(x, w, o)
-    with pytest.raises(Exception, match="ran out"):
+    for rows, n in ((256, 256), (20000, 512)):  # one block to a tile, two
+        o = offsets_of([rows])
+        x, w = normal(rows, 4096, t=torch.bfloat16, seed=1), normal(1, 4096, n, t=torch.bfloat16, seed=2)
+        want = scn.grouped_product(x, w, o)
         scn.poll_errors()
-    assert torch.equal(scn.grouped_product(x, w, o), want)
-    scn.poll_errors()
+        lib.scn_test_drop_barrier_arrival()
+        scn.grouped_product(x, w, o)
+        with pytest.raises(Exception, match="ran out"):
+            scn.poll_errors()
+        assert torch.equal(scn.grouped_product(x, w, o), want)
+        scn.poll_errors()
 
 
 def test_a_block_in_training(cuda):
