@@ -58,7 +58,7 @@ struct GroupParams {
   int stages;
   unsigned idesc;          // without N
   void *out;
-  int out_type, vectors;   // vectors: a row of results takes 16-byte stores
+  int out_type, vectors, part_vectors;  // vectors_of the results and of the partial sums
   float *partial;          // weights: [unit of a group of several units][m][n]
   const void *bias;
   int bias_type;
@@ -206,23 +206,37 @@ __device__ __forceinline__ float value_at(const void *p, int type, long long i) 
                                      : __half2float(__ldg((const __half *)p + i));
 }
 
-// 32 results of a row from column c on
+// 32 results of a row from column c on.  vectors 2: whole sectors of 32 bytes (pieces of 16 bytes reach L2 as two writes of half
+// a sector: group_wide_8bit took 40 us more), 1: pieces of 16 bytes, 0: one by one.
+__device__ __forceinline__ void store8w(void *p, int vectors, const unsigned *w) {
+  if (vectors == 2) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
 __device__ __forceinline__ void store32(void *out, int type, int vectors, long long at, int left, const float (&v)[32]) {
   if (vectors && left >= 32) {
     if (type == SCN_TYPE_FLOAT32) {
-      float4 *q = reinterpret_cast<float4 *>((float *)out + at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      uint4 *q = reinterpret_cast<uint4 *>((unsigned short *)out + at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        unsigned w[4];
+        unsigned w[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = type == SCN_TYPE_BFLOAT16 ? pair(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __nv_bfloat16())
-                                           : pair(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __half());
-        q[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
+        store8w((float *)out + at + 8 * i, vectors, w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        unsigned w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[j] = type == SCN_TYPE_BFLOAT16 ? pair(v[16 * i + 2 * j], v[16 * i + 2 * j + 1], __nv_bfloat16())
+                                           : pair(v[16 * i + 2 * j], v[16 * i + 2 * j + 1], __half());
+        store8w((unsigned short *)out + at + 16 * i, vectors, w);
       }
     }
     return;
@@ -237,6 +251,12 @@ __device__ __forceinline__ void store32(void *out, int type, int vectors, long l
     else
       ((__half *)out)[at + i] = __float2half_rn(v[i]);
   }
+}
+
+// Values of `bytes` in rows of n: how store32 may write them (a row begins at a multiple of n, a run of 32 at a multiple of 32)
+__host__ __device__ inline int vectors_of(uintptr_t p, long long n, int bytes) {
+  const uintptr_t all = p | (uintptr_t)(n * bytes);
+  return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
 }
 
 // What belongs to a unit's columns and rows, read by a warp of the epilogue while the unit is still being summed: lane l has
@@ -289,7 +309,7 @@ __device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, co
     if (u.m0 + lane_row >= P.m) return;
     const bool part = u.part >= 0;
     const long long row = (part ? (long long)u.part : u.group) * P.m + u.m0 + lane_row;
-    store32(part ? (void *)P.partial : P.out, part ? (int)SCN_TYPE_FLOAT32 : P.out_type, part ? P.n % 4 == 0 : P.vectors, row * P.n + c,
+    store32(part ? (void *)P.partial : P.out, part ? (int)SCN_TYPE_FLOAT32 : P.out_type, part ? P.part_vectors : P.vectors, row * P.n + c,
             P.n - c, v);
     return;
   }
@@ -596,7 +616,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   constexpr int kPerStage = F8 ? 2 * kStageRows : kStageRows;
   auto steps_of = [&](const Unit &u) { return WEIGHTS ? (u.rows + kStageRows - 1) / kStageRows : u.group < P.groups ? (P.k + kPerStage - 1) / kPerStage : 0; };
   auto width_of = [&](const Unit &u) { return min(kPairN, (P.n - u.n0 + 31) / 32 * 32); };  // columns of the instruction
-  auto boxes_of = [&](const Unit &u, int r) { return WEIGHTS ? 2 : max(0, min(kTileM, u.rows - r * kTileM) + kBoxRows - 1) / kBoxRows; };
+  auto boxes_of = [&](const Unit &u, int r) { return WEIGHTS ? 2 : u.rows > r * kTileM; };  // copies of the left operand
 
   // ==== copies ====
   if (warp == 0) {
@@ -607,7 +627,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     for (long long i = pair; i < units && ok; i += pairs) {
       const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
       const int steps = steps_of(u), n0 = u.n0 + (int)rank * (width_of(u) / 2), boxes = boxes_of(u, rank);
-      constexpr unsigned kBox = WEIGHTS ? kStageRows * kRow : kBoxRows * kRow;
+      constexpr unsigned kBox = WEIGHTS ? kStageRows * kRow : kTileM * kRow;
       const unsigned mine = boxes * kBox + kBBytes, both = (boxes_of(u, 0) + boxes_of(u, 1)) * kBox + 2 * kBBytes;
       for (int k = 0; k < steps; ++k, ++step) {
         const int st = step % kStages;
@@ -630,7 +650,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             for (int j = 0; j < 2; ++j) load_tile_pair(a + j * kStageRows * kRow, &map_a, u.m0 + (int)rank * kTileM + 64 * j, u.row + k * kStageRows, 0, 0, bar);
             for (int j = 0; j < 2; ++j) load_tile_pair(b + j * kStageRows * kRow, &map_b, n0 + 64 * j, u.row + k * kStageRows, 0, 0, bar);
           } else {
-            for (int j = 0; j < boxes; ++j) load_tile_pair(a + j * kBoxRows * kRow, &map_a, k * kPerStage, u.row + (int)rank * kTileM + j * kBoxRows, 0, 0, bar);
+            if (boxes) load_tile_pair(a, &map_a, k * kPerStage, u.row + (int)rank * kTileM, 0, 0, bar);
             if (B_ROWS)
               for (int j = 0; j < 2; ++j) load_tile_pair(b + j * kStageRows * kRow, &map_b, n0 + 64 * j, k * kStageRows, u.group, 0, bar);
             else
@@ -1057,11 +1077,11 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(type, false, b_rows, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
-  P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
+  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_size), P.part_vectors = vectors_of(0, n, 4);
   P.bias = bias, P.bias_type = bias_type, P.row_scale = row_scale, P.col_scale = col_scale, P.drop = drop;
   const int per = f8 ? 128 : 64;
   CUtensorMap a, b;
-  SCN_TRY(make_map(&a, x, type, k, G.n_rows, parts, 1, per, kBoxRows));  // (parts lie where groups would)
+  SCN_TRY(make_map(&a, x, type, k, G.n_rows, parts, 1, per, pair ? kTileM : kBoxRows));  // (parts lie where groups would)
   SCN_TRY(b_rows ? make_map(&b, w, type, n, k, G.groups, parts, 64, 64) : make_map(&b, w, type, k, n, G.groups, parts, per, pair ? tn / 2 : tn));
   const long long most = (pair ? pair_tiles : row_tiles) * P.n_tiles;
   if (pair)
@@ -1109,7 +1129,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
   P.idesc = idesc_of(type, true, true, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
-  P.out = out, P.out_type = out_type, P.vectors = (uintptr_t)out % 16 == 0 && (long long)n * out_size % 16 == 0;
+  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_size), P.part_vectors = vectors_of(0, n, 4);
   const bool split = G.n_rows > P.chunk;
   // (a group of several units has more than P.chunk rows: at most n_rows / chunk of them, with one unit more each than that)
   if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * m * n));
