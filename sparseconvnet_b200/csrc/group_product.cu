@@ -149,23 +149,37 @@ __device__ __forceinline__ void scan_groups(const GroupParams &P, Shared &S) {
   __syncthreads();
 }
 
+// Units in rising order: a role walks its block's units, so the next unit's group is looked for from the present one on (a step
+// or two, else by halves).  Between two units every role has this to do before it can go on: with a search over all groups
+// and a 64-bit division it took some 800 cycles.
 template <bool WEIGHTS, int TN>
-__device__ __forceinline__ Unit unit_at(const GroupParams &P, const Shared &S, long long u) {
-  const int all = WEIGHTS ? P.groups : P.groups + 2;
-  const int tiles = WEIGHTS ? P.n_tiles * P.m_tiles : P.n_tiles;
-  const int r = (int)(u / tiles), t = (int)(u - (long long)r * tiles);
-  int lo = 0, hi = all - 1;  // the last group that begins at or before r: groups without a unit share their start with the next
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (S.first[mid] <= r)
-      lo = mid;
-    else
-      hi = mid - 1;
+struct Walk {
+  const GroupParams &P;
+  const Shared &S;
+  int group = 0;
+  __device__ __forceinline__ Walk(const GroupParams &p, const Shared &s) : P(p), S(s) {}
+  __device__ __forceinline__ Unit at(long long u) {
+    const int all = WEIGHTS ? P.groups : P.groups + 2;
+    const int tiles = WEIGHTS ? P.n_tiles * P.m_tiles : P.n_tiles;
+    const int r = u >> 32 ? (int)(u / tiles) : (int)((unsigned)u / (unsigned)tiles), t = (int)(u - (long long)r * tiles);
+    for (int i = 0; i < 3 && S.first[group + 1] <= r; ++i) ++group;  // (first[all] is above every r)
+    if (S.first[group + 1] <= r) {
+      int lo = group + 1, hi = all - 1;  // the last group that begins at or before r: one without a unit shares its start with the next
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (S.first[mid] <= r)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      group = lo;
+    }
+    const int each = WEIGHTS ? P.chunk : P.tile, row = S.begin[group] + (r - S.first[group]) * each;
+    const int m = WEIGHTS ? (int)((unsigned)t / (unsigned)P.n_tiles) : 0;
+    return {group, row, min(each, S.end[group] - row), (t - m * P.n_tiles) * TN, m * P.tile,
+            WEIGHTS && S.part[group] >= 0 ? S.part[group] + r - S.first[group] : -1};
   }
-  const int each = WEIGHTS ? P.chunk : P.tile, row = S.begin[lo] + (r - S.first[lo]) * each;
-  return {lo, row, min(each, S.end[lo] - row), (WEIGHTS ? t % P.n_tiles : t) * TN, WEIGHTS ? t / P.n_tiles * P.tile : 0,
-          WEIGHTS && S.part[lo] >= 0 ? S.part[lo] + r - S.first[lo] : -1};
-}
+};
 
 __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w, unsigned long long *bar) {
   asm volatile(
@@ -352,8 +366,9 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const bool lead = elect_one();
     int step = 0;
     bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
     for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
-      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const Unit u = walk.at(i);
       const int steps = steps_of(u);
       const int a_boxes = WEIGHTS ? 2 : (u.rows + kBoxRows - 1) / kBoxRows;
       const unsigned bytes = PARTS * ((WEIGHTS ? kABytes : a_boxes * kBoxRows * kRow) + kBBytes);
@@ -390,8 +405,9 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const unsigned lead = elect_one();
     int step = 0, turn = 0;
     bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
     for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
-      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const Unit u = walk.at(i);
       const int steps = steps_of(u);
       const unsigned idesc = P.idesc | (unsigned)(min(TN, (P.n - u.n0 + 15) / 16 * 16) >> 3) << 17;
       for (int k = 0; k < steps; ++k, ++step) {
@@ -447,8 +463,9 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const int lane_row = quarter * 32 + lane;
     int turn = 0;
     bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
     for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
-      const Unit u = unit_at<WEIGHTS, TN>(P, S, i);
+      const Unit u = walk.at(i);
       const int steps = steps_of(u), columns = min(P.n - u.n0 - half * kMine, kMine);
       const int turns = steps == 0 ? 0 : SUMS ? (steps + kDrain - 1) / kDrain : 1;
       Terms<kMine, WEIGHTS, F8> terms;
@@ -624,8 +641,9 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     int step = 0;
     unsigned tails = 0;  // a bit per stage, the other way round after each sum that ended there
     bool ok = true;
+    Walk<WEIGHTS, kPairN> walk(P, S);
     for (long long i = pair; i < units && ok; i += pairs) {
-      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const Unit u = walk.at(i);
       const int steps = steps_of(u), n0 = u.n0 + (int)rank * (width_of(u) / 2), boxes = boxes_of(u, rank);
       constexpr unsigned kBox = WEIGHTS ? kStageRows * kRow : kTileM * kRow;
       const unsigned mine = boxes * kBox + kBBytes, both = (boxes_of(u, 0) + boxes_of(u, 1)) * kBox + 2 * kBBytes;
@@ -670,8 +688,9 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     int step = 0, turn = 0;
     unsigned tails = 0;
     bool ok = true;
+    Walk<WEIGHTS, kPairN> walk(P, S);
     for (long long i = pair; i < units && ok; i += pairs) {
-      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const Unit u = walk.at(i);
       const int steps = steps_of(u);
       const unsigned idesc = P.idesc | (unsigned)(width_of(u) >> 3) << 17;
       const int behind = WEIGHTS ? u.rows % kStageRows : 0;
@@ -727,8 +746,9 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     const int lane_row = (int)rank * kTileM + quarter * 32 + lane;
     int turn = 0;
     bool ok = true;
+    Walk<WEIGHTS, kPairN> walk(P, S);
     for (long long i = pair; i < units && ok; i += pairs) {
-      const Unit u = unit_at<WEIGHTS, kPairN>(P, S, i);
+      const Unit u = walk.at(i);
       const int columns = min(P.n - u.n0 - half * kMine, kMine);
       const bool summed = steps_of(u) > 0;
       Terms<kMine, WEIGHTS, F8> terms;
@@ -874,8 +894,9 @@ k_group_bias(const __grid_constant__ GroupParams P, const void *d_out, long long
   __shared__ float part[8][33];
   scan_groups<true>(P, S);
   const int lane = threadIdx.x % 32, along = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+  Walk<true, 64> walk(P, S);
   for (long long u = blockIdx.y; u < S.first[P.groups]; u += gridDim.y) {
-    const Unit unit = unit_at<true, 64>(P, S, u);
+    const Unit unit = walk.at(u);
     float v = 0.f;
     if (c < P.n) {
       int r = along;
