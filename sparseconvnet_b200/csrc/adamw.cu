@@ -102,11 +102,7 @@ template <typename T, bool WHOLE>
 __device__ __forceinline__ void get8(const void *p, long long at, long long n, float (&v)[8]) {
   if (WHOLE) {
     unsigned w[Words<T>::N];
-#pragma unroll
-    for (int i = 0; i < Words<T>::N; i += 4) {
-      const uint4 q = load_stream((const unsigned *)((const T *)p + at) + i);
-      w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
-    }
+    load_words((const T *)p + at, w);
     unpack8(w, v, T());
   } else {
 #pragma unroll
@@ -118,9 +114,7 @@ __device__ __forceinline__ void put8(void *p, long long at, long long n, const f
   if (WHOLE) {
     unsigned w[Words<T>::N];
     pack8(v, w, T());
-#pragma unroll
-    for (int i = 0; i < Words<T>::N; i += 4)
-      __stcs(reinterpret_cast<uint4 *>((unsigned *)((T *)p + at) + i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+    store_words((T *)p + at, w);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -282,7 +276,7 @@ int launch(const scn_adamw_tensor *tensors, int64_t n, Step A, cudaStream_t stre
       if (t.n == 0) continue;
       bool aligned = true;
       for (const void *p : {(const void *)t.param, t.grad, (const void *)t.exp_avg, (const void *)t.exp_avg_sq, (const void *)t.copy})
-        aligned = aligned && (uintptr_t)p % 16 == 0;
+        aligned = aligned && (uintptr_t)p % 32 == 0;
       T.e[A.count++] = {t.param, t.exp_avg, t.exp_avg_sq, t.copy, t.grad, t.exp_avg_scale, t.exp_avg_sq_scale, t.n, first * 2 + aligned};
       first += blocks_of(t.n);
     }

@@ -41,31 +41,42 @@ struct NormBackParams {
   int planes, dy_type, lanes;
 };
 
-// Sum (or maximum, of bit patterns of non-negative floats: a NaN's are above all numbers') over the `lanes` threads of a row.
-// `turn` alternates between two buffers, so that one barrier per sum is enough.
+// max(a, |b|); a NaN is above all numbers
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("{.reg .f32 t; abs.f32 t, %2; max.NaN.f32 %0, %1, t;}" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// `sum`, and with MAX `most`, over the `lanes` threads of a row.  `turn` alternates between two buffers, so that one barrier is
+// enough.
 template <bool MAX>
-__device__ __forceinline__ float over_row(float v, int lanes, float *shared, int &turn) {
+__device__ __forceinline__ void over_row(float &sum, float &most, int lanes, float2 *shared, int &turn) {
   const unsigned full = 0xffffffffu;
   const int within = lanes < 32 ? lanes : 32;
   for (int d = within >> 1; d; d >>= 1) {
-    const float o = __shfl_xor_sync(full, v, d);
-    v = MAX ? __uint_as_float(max(__float_as_uint(v), __float_as_uint(o))) : v + o;
+    sum += __shfl_xor_sync(full, sum, d);
+    if (MAX) most = larger(most, __shfl_xor_sync(full, most, d));
   }
-  if (lanes <= 32) return v;
-  float *buf = shared + (turn ^= 1) * (kMostLanes / 32);
+  if (lanes <= 32) return;
+  float2 *buf = shared + (turn ^= 1) * (kMostLanes / 32);
   const int warp = threadIdx.x / 32, per_row = lanes / 32;
-  if (threadIdx.x % 32 == 0) buf[warp] = v;
+  if (threadIdx.x % 32 == 0) buf[warp] = make_float2(sum, most);
   __syncthreads();
-  const float *mine = buf + warp / per_row * per_row;
-  v = mine[0];
-  for (int i = 1; i < per_row; ++i) v = MAX ? __uint_as_float(max(__float_as_uint(v), __float_as_uint(mine[i]))) : v + mine[i];
-  return v;
+  const float2 *mine = buf + warp / per_row * per_row;
+  sum = mine[0].x, most = mine[0].y;
+  for (int i = 1; i < per_row; ++i) {
+    const float2 v = mine[i];
+    sum += v.x;
+    if (MAX) most = larger(most, v.y);
+  }
 }
 
-template <int V>
+template <int V, bool QUANT>
 __device__ __forceinline__ void store_out(void *out, int type, long long row, int planes, int chunk, int lanes, int lane, const float (&y)[8]) {
   const long long at = row * planes;
-  if (type == SCN_TYPE_BFLOAT16) {
+  if (QUANT) {
+    store8_e4m3<V>((unsigned char *)out + at, planes, chunk, lanes, lane, y);
+  } else if (type == SCN_TYPE_BFLOAT16) {
     unsigned w[4];
     pack8(y, w, __nv_bfloat16());
     store8<__nv_bfloat16, V>((__nv_bfloat16 *)out + at, planes, chunk, lanes, lane, w);
@@ -73,17 +84,25 @@ __device__ __forceinline__ void store_out(void *out, int type, long long row, in
     unsigned w[8];
     pack8(y, w, 0.f);
     store8<float, V>((float *)out + at, planes, chunk, lanes, lane, w);
-  } else if (type == SCN_TYPE_FLOAT16) {
+  } else {
     unsigned w[4];
     pack8(y, w, __half());
     store8<__half, V>((__half *)out + at, planes, chunk, lanes, lane, w);
-  } else {
-    store8_e4m3<V>((unsigned char *)out + at, planes, chunk, lanes, lane, y);
   }
 }
 
 template <int V>
 __device__ __forceinline__ void load_weights(const float *w, int planes, int chunk, int lanes, int lane, float (&v)[8]) {
+  if (V == 8) {
+    const int c = place<8>(chunk, 0, lanes, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = w || c >= planes ? 0.f : 1.f;
+    if (w && c < planes) {
+      const float4 p = __ldg((const float4 *)(w + c)), q = __ldg((const float4 *)(w + c) + 1);
+      v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8 / V; ++j) {
     const int c = place<V>(chunk, j, lanes, lane);
@@ -92,15 +111,14 @@ __device__ __forceinline__ void load_weights(const float *w, int planes, int chu
   }
 }
 
-template <typename T, int V, int CH>
+template <typename T, int V, int CH, bool QUANT>
 __global__ void __launch_bounds__(kMostLanes)
 k_rms_norm(const NormParams P) {
   SCN_GRID_WAIT();
-  __shared__ float shared[2 * (kMostLanes / 32)];
+  __shared__ float2 shared[2 * (kMostLanes / 32)];
   const int lanes = P.lanes, lane = threadIdx.x % lanes, per_block = blockDim.x / lanes;
   const long long step = (long long)gridDim.x * per_block;
   long long row = (long long)blockIdx.x * per_block + threadIdx.x / lanes;
-  const bool quantized = P.out_type == SCN_TYPE_E4M3;
   int turn = 0;
   float w[CH][8];
 #pragma unroll
@@ -117,7 +135,7 @@ k_rms_norm(const NormParams P) {
   ask(row);
   for (long long first = (long long)blockIdx.x * per_block; first < P.n_rows; first += step, row += step) {
     const bool real = row < P.n_rows;
-    float s[CH][8], squares = 0.f;
+    float s[CH][8], squares = 0.f, most = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       unpack8(x[i], s[i], T());
@@ -132,33 +150,28 @@ k_rms_norm(const NormParams P) {
         if (real) store8<T, V>((T *)P.sum + row * P.planes, P.planes, i, lanes, lane, sw);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) squares = fmaf(s[i][j], s[i][j], squares);
+      for (int j = 0; j < 8; ++j) {
+        squares = fmaf(s[i][j], s[i][j], squares);
+        s[i][j] *= w[i][j];
+        if (QUANT) most = larger(most, s[i][j]);
+      }
     }
     ask(row + step);
-    const float k = __frsqrt_rn(over_row<false>(squares, lanes, shared, turn) / (float)P.planes + P.eps);
+    over_row<QUANT>(squares, most, lanes, shared, turn);
+    float k = __frsqrt_rn(squares / (float)P.planes + P.eps);
     if (P.inv_rms && lane == 0 && real) P.inv_rms[row] = k;
+    if (QUANT) {  // the largest |s w| k is the largest |y|: one pass over the row for both sums
+      most = larger(kSmallest, most * k);
+      if (lane == 0 && real) P.scale[row] = most / kE4m3Most;
+    }
+    const float per = QUANT ? kE4m3Most / most : 1.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * k * w[i][j];
-    if (quantized) {
-      float most = kSmallest;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(s[i][j]) & 0x7FFFFFFFu));
-      most = over_row<true>(most, lanes, shared, turn);
-      if (lane == 0 && real) P.scale[row] = most / kE4m3Most;
-      const float per = kE4m3Most / most;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] *= per;
-    }
+      for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * k * per;
     if (real) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) store_out<V>(P.out, P.out_type, row, P.planes, i, lanes, lane, s[i]);
+      for (int i = 0; i < CH; ++i) store_out<V, QUANT>(P.out, P.out_type, row, P.planes, i, lanes, lane, s[i]);
     }
   }
 }
@@ -183,63 +196,69 @@ __device__ __forceinline__ void load_any(const void *p, int type, long long row,
 
 // The weights' gradient: a thread keeps the sums of its planes over all rows of its block, the rows' groups of a block are
 // added in shared memory, the blocks' sums by k_add_blocks: a fixed order.
-template <typename T, int V, int CH>
+template <typename T, int V, int CH, bool SAME>
 __global__ void __launch_bounds__(kMostLanes)
 k_rms_norm_back(const NormBackParams P) {
   SCN_GRID_WAIT();
-  __shared__ float shared[2 * (kMostLanes / 32)];
+  __shared__ float2 shared[2 * (kMostLanes / 32)];
   extern __shared__ float sums[];  // [rows of a block][planes]
   const int lanes = P.lanes, lane = threadIdx.x % lanes, per_block = blockDim.x / lanes;
   const long long step = (long long)gridDim.x * per_block;
   long long row = (long long)blockIdx.x * per_block + threadIdx.x / lanes;
   int turn = 0;
-  float w[CH][8], dw[CH][8];
+  float dw[CH][8];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    load_weights<V>(P.w, P.planes, i, lanes, lane, w[i]);
+  for (int i = 0; i < CH; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
-  }
+  // the next row on its way (a gradient of another type than the rows' is read when it is needed)
+  unsigned sw[CH][Words<T>::N], dyw[CH][Words<T>::N], dsw[CH][Words<T>::N];
+  float k_next = 0.f;
+  auto ask = [&](long long at) {
+    const int n = at < P.n_rows ? P.planes : 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      load8<T, V>((const T *)P.s + at * P.s_stride, n, i, lanes, lane, sw[i]);
+      if (SAME) load8<T, V>((const T *)P.dy + at * P.planes, n, i, lanes, lane, dyw[i]);
+      if (P.ds) load8<T, V>((const T *)P.ds + at * P.planes, n, i, lanes, lane, dsw[i]);
+    }
+    k_next = n ? __ldg(P.inv_rms + at) : 0.f;
+  };
+  ask(row);
   for (long long first = (long long)blockIdx.x * per_block; first < P.n_rows; first += step, row += step) {
     const bool real = row < P.n_rows;
-    const int n = real ? P.planes : 0;
-    unsigned sw[CH][Words<T>::N], ow[CH][Words<T>::N];
-    float d[CH][8], along = 0.f;
+    const float k = k_next;
+    float h[CH][8], d[CH][8], o[CH][8], along = 0.f, none = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      load8<T, V>((const T *)P.s + row * P.s_stride, n, i, lanes, lane, sw[i]);
-      load_any<V>(P.dy, P.dy_type, row, P.planes, n, i, lanes, lane, d[i]);
-    }
-    if (P.ds)
-#pragma unroll
-      for (int i = 0; i < CH; ++i) load8<T, V>((const T *)P.ds + row * P.planes, n, i, lanes, lane, ow[i]);
-    const float k = real ? __ldg(P.inv_rms + row) : 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      float s[8];
-      unpack8(sw[i], s, T());
+      float w[8];
+      load_weights<V>(P.w, P.planes, i, lanes, lane, w);
+      unpack8(sw[i], h[i], T());
+      if (SAME)
+        unpack8(dyw[i], d[i], T());
+      else
+        load_any<V>(P.dy, P.dy_type, row, P.planes, real ? P.planes : 0, i, lanes, lane, d[i]);
+      if (P.ds) unpack8(dsw[i], o[i], T());
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float h = s[j] * k;
-        dw[i][j] = fmaf(d[i][j], h, dw[i][j]);
-        d[i][j] *= w[i][j];
-        along = fmaf(d[i][j], h, along);
+        h[i][j] *= k;
+        dw[i][j] = fmaf(d[i][j], h[i][j], dw[i][j]);
+        d[i][j] *= w[j];
+        along = fmaf(d[i][j], h[i][j], along);
       }
     }
-    along = over_row<false>(along, lanes, shared, turn) / (float)P.planes;
+    ask(row + step);
+    over_row<false>(along, none, lanes, shared, turn);
+    along /= (float)P.planes;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      float s[8], o[8];
-      unpack8(sw[i], s, T());
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = k * (d[i][j] - s[j] * k * along);
-      if (P.ds) {
-        unpack8(ow[i], o, T());
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] += o[j];
+      for (int j = 0; j < 8; ++j) {
+        h[i][j] = k * (d[i][j] - h[i][j] * along);
+        if (P.ds) h[i][j] += o[i][j];
       }
       unsigned q[Words<T>::N];
-      pack8(s, q, T());
+      pack8(h[i], q, T());
       if (real) store8<T, V>((T *)P.dx + row * P.planes, P.planes, i, lanes, lane, q);
     }
   }
@@ -303,35 +322,32 @@ __device__ __forceinline__ float rounded(float v, int type) {
 __global__ void __launch_bounds__(kMostLanes)
 k_rms_norm_long(const NormParams P, int type) {
   SCN_GRID_WAIT();
-  __shared__ float shared[2 * (kMostLanes / 32)];
+  __shared__ float2 shared[2 * (kMostLanes / 32)];
   int turn = 0;
   for (long long row = blockIdx.x; row < P.n_rows; row += gridDim.x) {
     auto value = [&](int c) {
       const float v = any_value(P.x, type, row * P.x_stride + c);
       return P.r ? rounded(v + any_value(P.r, type, row * P.r_stride + c), type) : v;
     };
-    float squares = 0.f;
+    float squares = 0.f, most = 0.f;
     for (int c = threadIdx.x; c < P.planes; c += kMostLanes) {
       const float s = value(c);
       squares = fmaf(s, s, squares);
+      most = larger(most, s * (P.w ? __ldg(P.w + c) : 1.f));
     }
-    const float k = __frsqrt_rn(over_row<false>(squares, kMostLanes, shared, turn) / (float)P.planes + P.eps);
+    over_row<true>(squares, most, kMostLanes, shared, turn);
+    const float k = __frsqrt_rn(squares / (float)P.planes + P.eps);
     if (P.inv_rms && threadIdx.x == 0) P.inv_rms[row] = k;
     float per = 1.f;
     if (P.out_type == SCN_TYPE_E4M3) {
-      float most = kSmallest;
-      for (int c = threadIdx.x; c < P.planes; c += kMostLanes) {
-        const float y = value(c) * k * (P.w ? __ldg(P.w + c) : 1.f);
-        most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(y) & 0x7FFFFFFFu));
-      }
-      most = over_row<true>(most, kMostLanes, shared, turn);
+      most = larger(kSmallest, most * k);
       if (threadIdx.x == 0) P.scale[row] = most / kE4m3Most;
       per = kE4m3Most / most;
     }
     for (int c = threadIdx.x; c < P.planes; c += kMostLanes) {
       const float s = value(c);
       if (P.r) store_value(P.sum, type, row * P.planes + c, s);
-      store_value(P.out, P.out_type, row * P.planes + c, s * k * (P.w ? __ldg(P.w + c) : 1.f) * per);
+      store_value(P.out, P.out_type, row * P.planes + c, s * (P.w ? __ldg(P.w + c) : 1.f) * k * per);
     }
   }
 }
@@ -339,7 +355,7 @@ k_rms_norm_long(const NormParams P, int type) {
 __global__ void __launch_bounds__(kMostLanes)
 k_rms_norm_back_long(const NormBackParams P, int type) {
   SCN_GRID_WAIT();
-  __shared__ float shared[2 * (kMostLanes / 32)];
+  __shared__ float2 shared[2 * (kMostLanes / 32)];
   int turn = 0;
   for (long long row = blockIdx.x; row < P.n_rows; row += gridDim.x) {
     const float k = __ldg(P.inv_rms + row);
@@ -347,7 +363,9 @@ k_rms_norm_back_long(const NormBackParams P, int type) {
     for (int c = threadIdx.x; c < P.planes; c += kMostLanes)
       along = fmaf(any_value(P.dy, P.dy_type, row * P.planes + c) * (P.w ? __ldg(P.w + c) : 1.f),
                    any_value(P.s, type, row * P.s_stride + c) * k, along);
-    along = over_row<false>(along, kMostLanes, shared, turn) / (float)P.planes;
+    float none = 0.f;
+    over_row<false>(along, none, kMostLanes, shared, turn);
+    along /= (float)P.planes;
     for (int c = threadIdx.x; c < P.planes; c += kMostLanes) {
       const float t = any_value(P.dy, P.dy_type, row * P.planes + c) * (P.w ? __ldg(P.w + c) : 1.f);
       float v = k * (t - any_value(P.s, type, row * P.s_stride + c) * k * along);
@@ -369,13 +387,21 @@ k_rms_norm_weights_long(const NormBackParams P, int type) {
   P.partial[(long long)blockIdx.y * P.planes + c] = v;
 }
 
-// How a row lies in registers: `lanes` threads of `chunks` times 8 values with the fewest places left over; 4 chunks, which
-// do not fit the registers without spilling, only where nothing else is as good.  False: the row does not fit.
-bool shape_of(int planes, int *lanes, int *chunks) {
+// How a row lies in registers: `lanes` threads of `chunks` times 8 values with the fewest places left over, and among equals
+// by what measured best (GB/s of 6548, forward 16384 x 4096 bf16: 4 chunks 6230, 2 5520, 1 5490; in 8 bits 6230, 5190, 4450; of
+// 400000 x 32: 4700, 5510, 6010; 8192 x 4096 fp32: 2 chunks 5810, 1 5620, 4 5600; backward 16384 x 4096 bf16: 2 chunks 4180, 1
+// 3250, 4 2000 (spills); 8192 x 4096 fp32: 1 chunk 5960, 2 5310; 267011 x 96
+// fp32: 1 chunk 5860, 3 4180).  Rows of a few chunks are spread, so that a warp's loads are
+// dense; long rows are held by as few threads as their registers allow, because each row costs all its threads a barrier.
+bool shape_of(int planes, int type, bool backward, int *lanes, int *chunks) {
   const int need = (int)ceil_div(planes, 8);
+  const bool wide = type == SCN_TYPE_FLOAT32;
+  static const int orders[5][4] = {{1, 2, 3, 4}, {2, 1, 3, 4}, {4, 3, 2, 1}, {1, 2, 3, 4}, {2, 1, 3, 4}};
+  const int *order = orders[backward ? (wide ? 3 : 4) : need <= 8 ? 0 : wide ? 1 : 2];
   int best = 0;
-  for (const int ch : {2, 3, 1, 4}) {
-    const int l = (int)next_pow2((unsigned long long)ceil_div(need, ch));
+  for (int i = 0; i < 4; ++i) {
+    if (backward && best && i == 2) break;  // 3 and 4 chunks spill there: rows of over 8192 planes only
+    const int ch = order[i], l = (int)next_pow2((unsigned long long)ceil_div(need, ch));
     if (l > kMostLanes) continue;
     if (!best || l * ch < best) best = l * ch, *lanes = l, *chunks = ch;
   }
@@ -391,8 +417,8 @@ struct Vectors {
   void add(const void *p, int type, long long stride, int planes) {
     if (!p) return;
     const int size = size_of(type);
-    auto fits = [&](int n) {  // (8 fp32 values are two vectors of 16 bytes)
-      const uintptr_t bytes = (uintptr_t)std::min(16, n * size);
+    auto fits = [&](int n) {
+      const uintptr_t bytes = (uintptr_t)(n * size);
       return (uintptr_t)p % bytes == 0 && (uintptr_t)(stride * size) % bytes == 0 && planes % n == 0;
     };
     if (v == 8 && !fits(8)) v = 2;
@@ -404,15 +430,16 @@ template <typename T, int V>
 int launch_forward(const NormParams &P, int chunks, cudaStream_t stream) {
   const int threads = std::max(kThreads, P.lanes);
   const long long need = ceil_div(P.n_rows, threads / P.lanes);
-#define SCN_NORM(CH)                                                                                          \
-  case CH: {                                                                                                  \
+#define SCN_NORM(CH, Q)                                                                                       \
+  case CH * 2 + Q: {                                                                                          \
     int most = 0;                                                                                             \
-    SCN_TRY((resident_blocks<k_rms_norm<T, V, CH>>(threads, 0, &most)));                                        \
-    SCN_LAUNCH((k_rms_norm<T, V, CH>), (unsigned)std::min<long long>(need, most), threads, 0, stream, P);     \
+    SCN_TRY((resident_blocks<k_rms_norm<T, V, CH, Q>>(threads, 0, &most)));                                   \
+    SCN_LAUNCH((k_rms_norm<T, V, CH, Q>), (unsigned)std::min<long long>(need, most), threads, 0, stream, P);  \
     break;                                                                                                    \
   }
-  switch (chunks) {
-    SCN_NORM(1) SCN_NORM(2) SCN_NORM(3) SCN_NORM(4)
+  switch (chunks * 2 + (P.out_type == SCN_TYPE_E4M3)) {
+    SCN_NORM(1, false) SCN_NORM(2, false) SCN_NORM(3, false) SCN_NORM(4, false)
+    SCN_NORM(1, true) SCN_NORM(2, true) SCN_NORM(3, true) SCN_NORM(4, true)
   }
 #undef SCN_NORM
   SCN_CUDA_CHECK(cudaGetLastError());
@@ -425,8 +452,8 @@ int add_blocks(const float *partial, long long blocks, int planes, float *out, c
   return SCN_OK;
 }
 
-template <typename T, int V>
-int launch_backward(NormBackParams P, int chunks, float *d_weight, cudaStream_t stream) {
+template <typename T, int V, bool SAME>
+int launch_back(NormBackParams P, int chunks, float *d_weight, cudaStream_t stream) {
   const int threads = std::max(kThreads, P.lanes);
   const long long need = ceil_div(P.n_rows, threads / P.lanes);
   const size_t smem = d_weight ? sizeof(float) * (size_t)(threads / P.lanes) * P.planes : 0;
@@ -436,12 +463,12 @@ int launch_backward(NormBackParams P, int chunks, float *d_weight, cudaStream_t 
   case CH: {                                                                                                   \
     int most = 0;                                                                                              \
     if (smem > 48 * 1024)                                                                                      \
-      SCN_CUDA_CHECK(cudaFuncSetAttribute(k_rms_norm_back<T, V, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+      SCN_CUDA_CHECK(cudaFuncSetAttribute(k_rms_norm_back<T, V, CH, SAME>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
                                           (int)smem));                                                         \
-    SCN_TRY((resident_blocks<k_rms_norm_back<T, V, CH>>(threads, 0, &most)));                                  \
+    SCN_TRY((resident_blocks<k_rms_norm_back<T, V, CH, SAME>>(threads, 0, &most)));                                  \
     blocks = std::min<long long>(need, most);                                                                  \
     if (d_weight) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)blocks * P.planes));                 \
-    SCN_LAUNCH((k_rms_norm_back<T, V, CH>), (unsigned)blocks, threads, smem, stream, P);                       \
+    SCN_LAUNCH((k_rms_norm_back<T, V, CH, SAME>), (unsigned)blocks, threads, smem, stream, P);                       \
     break;                                                                                                     \
   }
   switch (chunks) {
@@ -450,6 +477,12 @@ int launch_backward(NormBackParams P, int chunks, float *d_weight, cudaStream_t 
 #undef SCN_NORM
   SCN_CUDA_CHECK(cudaGetLastError());
   return d_weight ? add_blocks(P.partial, blocks, P.planes, d_weight, stream) : SCN_OK;
+}
+
+// (a gradient of another type than the rows' takes the form for any alignment)
+template <typename T, int V>
+int launch_backward(const NormBackParams &P, int chunks, float *d_weight, bool same, cudaStream_t stream) {
+  return same ? launch_back<T, V, true>(P, chunks, d_weight, stream) : launch_back<T, 1, false>(P, chunks, d_weight, stream);
 }
 
 #define SCN_BY_TYPE(call, type, v, ...)                                                                        \
@@ -481,7 +514,7 @@ int scn_rms_norm_forward(const void *x, int64_t x_stride, const void *residual, 
   SCN_REQUIRE((out_type == SCN_TYPE_E4M3) == (scale != nullptr), SCN_ERR_BAD_ARG, "rms_norm: scales belong to 8-bit results");
   NormParams P{x, residual, weight, sum, out, scale, inv_rms, n_rows, x_stride, residual_stride, n_planes, out_type, 0, (float)eps};
   int chunks = 0;
-  if (!shape_of(n_planes, &P.lanes, &chunks)) {
+  if (!shape_of(n_planes, type, false, &P.lanes, &chunks)) {
     int most = 0;
     SCN_TRY(resident_blocks<k_rms_norm_long>(kMostLanes, 0, &most));
     SCN_LAUNCH(k_rms_norm_long, (unsigned)std::min<long long>(n_rows, most), kMostLanes, 0, stream, P, type);
@@ -493,6 +526,7 @@ int scn_rms_norm_forward(const void *x, int64_t x_stride, const void *residual, 
   vec.add(residual, type, residual_stride, n_planes);
   vec.add(sum, type, n_planes, n_planes);
   vec.add(out, out_type, n_planes, n_planes);
+  vec.add(weight, SCN_TYPE_FLOAT32, n_planes, n_planes);
   return SCN_BY_TYPE(launch_forward, type, vec.v, P, chunks, stream);
 }
 
@@ -509,7 +543,7 @@ int scn_rms_norm_backward(const void *s, int64_t s_stride, int type, const float
   SCN_REQUIRE(s && inv_rms && d_out && d_x, SCN_ERR_BAD_ARG, "rms_norm: null argument");
   NormBackParams P{s, d_out, d_sum, weight, inv_rms, d_x, nullptr, n_rows, s_stride, n_planes, d_out_type, 0};
   int chunks = 0;
-  if (!shape_of(n_planes, &P.lanes, &chunks)) {
+  if (!shape_of(n_planes, type, true, &P.lanes, &chunks)) {
     int most = 0;
     SCN_TRY(resident_blocks<k_rms_norm_back_long>(kMostLanes, 0, &most));
     SCN_LAUNCH(k_rms_norm_back_long, (unsigned)std::min<long long>(n_rows, most), kMostLanes, 0, stream, P, type);
@@ -527,7 +561,8 @@ int scn_rms_norm_backward(const void *s, int64_t s_stride, int type, const float
   vec.add(d_out, d_out_type, n_planes, n_planes);
   vec.add(d_sum, type, n_planes, n_planes);
   vec.add(d_x, type, n_planes, n_planes);
-  return SCN_BY_TYPE(launch_backward, type, vec.v, P, chunks, d_weight, stream);
+  vec.add(weight, SCN_TYPE_FLOAT32, n_planes, n_planes);
+  return SCN_BY_TYPE(launch_backward, type, vec.v, P, chunks, d_weight, type == d_out_type, stream);
 }
 
 }  // extern "C"

@@ -51,11 +51,23 @@ __device__ __forceinline__ void pack8(const float (&v)[8], unsigned (&w)[8], flo
   for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
 }
 
-// Streams that are read and written once: past L1, first to leave L2.
-__device__ __forceinline__ uint4 load_stream(const void *p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
+// N words of a stream that is read or written once, past L1.  8 words are one access of 32 bytes, a whole sector: as two of
+// 16 bytes the neighbouring lanes' accesses lie 32 bytes apart, and every sector is asked for twice.
+__device__ __forceinline__ void load_words(const void *p, unsigned (&w)[4]) {
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+}
+__device__ __forceinline__ void load_words(const void *p, unsigned (&w)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store_words(void *p, const unsigned (&w)[4]) {
+  __stcs(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
+}
+__device__ __forceinline__ void store_words(void *p, const unsigned (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+               "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // 8 values of a row as words, in vectors of V.  Vector j of thread `lane` of `lanes` holds the values from `at(j)` on, so
@@ -70,13 +82,7 @@ __device__ __forceinline__ void load8(const T *__restrict__ row, int n, int chun
     const int c = place<8>(chunk, 0, lanes, lane);
 #pragma unroll
     for (int i = 0; i < Words<T>::N; ++i) w[i] = 0;
-    if (c < n) {
-#pragma unroll
-      for (int i = 0; i < Words<T>::N; i += 4) {
-        const uint4 q = load_stream((const unsigned *)(row + c) + i);
-        w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
-      }
-    }
+    if (c < n) load_words(row + c, w);
   } else {
 #pragma unroll
     for (int j = 0; j < 8 / V; ++j) {
@@ -98,11 +104,7 @@ template <typename T, int V>
 __device__ __forceinline__ void store8(T *row, int n, int chunk, int lanes, int lane, const unsigned (&w)[Words<T>::N]) {
   if (V == 8) {
     const int c = place<8>(chunk, 0, lanes, lane);
-    if (c < n) {
-#pragma unroll
-      for (int i = 0; i < Words<T>::N; i += 4)
-        __stcs(reinterpret_cast<uint4 *>((unsigned *)(row + c) + i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
-    }
+    if (c < n) store_words(row + c, w);
   } else {
 #pragma unroll
     for (int j = 0; j < 8 / V; ++j) {
