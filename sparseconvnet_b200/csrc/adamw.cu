@@ -42,7 +42,7 @@ struct Step {
   unsigned long long *word;  // steps done; blocks that have ended above bit 40
   const float *lr_dev;       // may be null
   double log_b1, log_b2;
-  float lr, b1, b2, one_minus_b1, one_minus_b2, eps, wd;
+  float lr, b1, b2, one_minus_b1, one_minus_b2, eps, wd, one;
   unsigned seed;
   int grad_type, copy_type;  // copy_type -1: none
   int count;                 // tensors of this launch
@@ -56,15 +56,52 @@ __device__ __forceinline__ unsigned mixed(unsigned v) {  // the 32-bit finaliser
   return v ^ (v >> 16);
 }
 
-// 16 random bits as a number in [0, 1)
-__device__ __forceinline__ float chance(unsigned bits16) { return __uint_as_float(0x3F800000u | bits16 << 7) - 1.f; }
+// Two floats in a pair of registers: the FMA pipe takes both in one instruction.
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ void apart(Two t, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v)); }
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two add2_down(Two a, Two b) {
+  Two r;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 
-// |y| <= 448 (and what rounding adds) to the multiple of its binade's step below |y| + u step, u < 1: one of its two neighbours
-// among the values of e4m3.  The addition of 2^23 steps, rounded down, drops what lies below a step.
-__device__ __forceinline__ float to_neighbour(float y, float u) {
-  const unsigned e = max(__float_as_uint(y) & 0x7F800000u, 121u << 23);  // the exponent, at least -6
-  const float step = __uint_as_float(e - (3u << 23)), steps = __uint_as_float(e + (20u << 23));
-  return __fadd_rd(fmaf(u, step, fabsf(y)), steps) - steps;
+// The 16 bits of two hashes, lower or upper halves, as numbers 0 .. 65535
+template <bool UPPER>
+__device__ __forceinline__ Two chances(unsigned a, unsigned b) {  // (2^23 + bits) - 2^23
+  const unsigned pick = UPPER ? 0x7632u : 0x7610u;
+  return two(__uint_as_float(__byte_perm(a, 0x4B000000u, pick)), __uint_as_float(__byte_perm(b, 0x4B000000u, pick))) + two(-8388608.f);
+}
+
+// |y| <= 448 (and what rounding adds) to the multiples of their binades' steps below |y| + chance / 65536 steps: one of the two
+// neighbours among the values of e4m3.  The addition of 2^23 steps, rounded down, drops what lies below a step.
+__device__ __forceinline__ Two to_neighbours(float a, float b, Two chance) {
+  const float ea = fmaxf(__uint_as_float(__float_as_uint(a) & 0x7F800000u), 0x1p-6f), eb = fmaxf(__uint_as_float(__float_as_uint(b) & 0x7F800000u), 0x1p-6f);
+  const Two e = two(ea, eb), steps = e * two(0x1p20f);
+  const Two sum = fma2(chance, e * two(0x1p-19f), two(fabsf(a), fabsf(b)));
+  return add2_down(sum, steps) + steps * two(-1.f);
 }
 
 __device__ __forceinline__ float larger(float a, float b) {  // max(a, |b|); a NaN is above all numbers
@@ -81,7 +118,7 @@ __device__ __forceinline__ void from_e4m3(const uint2 q, float scale, float (&v)
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? q.x : q.y) >> (i % 2 * 16)), __NV_E4M3);
     const float2 f = __half22float2(__half2(h));
-    v[2 * i] = f.x * scale, v[2 * i + 1] = f.y * scale;
+    apart(two(f.x, f.y) * two(scale), v[2 * i], v[2 * i + 1]);
   }
 }
 
@@ -168,17 +205,25 @@ __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long lo
     get8<float, WHOLE>(E.m, first, E.n, m);
     get8<float, WHOLE>(E.v, first, E.n, r);
   }
-  const float keep = 1.f - A.wd;
+  const Two b1 = two(A.b1), b2 = two(A.b2), c1 = two(A.one_minus_b1), c2 = two(A.one_minus_b2), keep = two(1.f - A.wd);
+  // The roundings of the formula as it is written: a sum of products that came out one unit apart would be rounded to the
+  // other neighbour now and then.  Pairs' mul.rn and add.rn do get contracted; times one, which the compiler cannot see, not.
+  const Two one = two(A.one);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {  // (the roundings of the formula as it is written: no contraction)
-    const float v = BITS == 8 ? __fmul_rn(r[j], r[j]) : r[j];
-    m[j] = __fadd_rn(__fmul_rn(m[j], A.b1), __fmul_rn(g[j], A.one_minus_b1));
-    const float now = __fadd_rn(__fmul_rn(v, A.b2), __fmul_rn(__fmul_rn(g[j], g[j]), A.one_minus_b2));
-    const float root = __fsqrt_rn(now);
-    float per;  // (1 / x to a unit in the last place; eps keeps x above the subnormal numbers)
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per) : "f"(fmaf(root, per_root, A.eps)));
-    p[j] = fmaf(-rate * m[j], per, p[j] * keep);
-    r[j] = BITS == 8 ? root : now;
+  for (int j = 0; j < 8; j += 2) {
+    const Two gg = two(g[j], g[j + 1]), rr = two(r[j], r[j + 1]);
+    const Two mm = fma2(two(m[j], m[j + 1]) * b1, one, gg * c1);
+    const Two vv = fma2((BITS == 8 ? rr * rr : rr) * b2, one, (gg * gg) * c2);
+    float v0, v1, x0, x1;
+    apart(vv, v0, v1);
+    apart(mm, m[j], m[j + 1]);
+    const float r0 = __fsqrt_rn(v0), r1 = __fsqrt_rn(v1);
+    apart(fma2(two(r0, r1), two(per_root), two(A.eps)), x0, x1);
+    // (1 / x to a unit in the last place; eps keeps x above the subnormal numbers)
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x1));
+    apart(fma2(mm * two(-rate), two(x0, x1), two(p[j], p[j + 1]) * keep), p[j], p[j + 1]);
+    r[j] = BITS == 8 ? r0 : v0, r[j + 1] = BITS == 8 ? r1 : v1;
   }
   put8<P, WHOLE>(E.p, first, E.n, p);
   if (A.copy_type == SCN_TYPE_BFLOAT16)
@@ -203,14 +248,18 @@ __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long lo
     E.v_scale[at] = __fmul_rn(most_r, 1.f / kE4m3Most);
   }
   const float per_m = __fmul_rn(__frcp_rn(most_m), kE4m3Most), per_r = __fmul_rn(__frcp_rn(most_r), kE4m3Most);
-  const unsigned low = (unsigned)(number * kBlock), high = (unsigned)(number * kBlock >> 32);
+  const unsigned low = (unsigned)(number * kBlock) + (WHOLE ? lane * 8 : lane), high = (unsigned)(number * kBlock >> 32);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const unsigned bits = mixed(mixed((low + (WHOLE ? lane * 8 + j : lane + 32 * j)) ^ key) ^ high);
-    const float ym = __fmul_rn(m[j], per_m), yr = __fmul_rn(r[j], per_r);
-    m[j] = copysignf(to_neighbour(ym, chance(bits & 0xFFFFu)), ym);
-    r[j] = to_neighbour(yr, chance(bits >> 16));
-    if (yr > 0.f) r[j] = fmaxf(r[j], kE4m3Least);
+  for (int j = 0; j < 8; j += 2) {
+    const unsigned h0 = mixed(mixed((low + (WHOLE ? j : 32 * j)) ^ key) ^ high), h1 = mixed(mixed((low + (WHOLE ? j + 1 : 32 * j + 32)) ^ key) ^ high);
+    float a, b, c, d;
+    apart(two(m[j], m[j + 1]) * two(per_m), a, b);
+    apart(two(r[j], r[j + 1]) * two(per_r), c, d);
+    apart(to_neighbours(a, b, chances<false>(h0, h1)), m[j], m[j + 1]);
+    apart(to_neighbours(c, d, chances<true>(h0, h1)), r[j], r[j + 1]);
+    m[j] = copysignf(m[j], a), m[j + 1] = copysignf(m[j + 1], b);
+    if (c > 0.f) r[j] = larger(kE4m3Least, r[j]);
+    if (d > 0.f) r[j + 1] = larger(kE4m3Least, r[j + 1]);
   }
   put8_e4m3<WHOLE>(E.m, first, E.n, m);
   put8_e4m3<WHOLE>(E.v, first, E.n, r);
@@ -332,7 +381,7 @@ extern "C" int scn_adamw_step(const scn_adamw_tensor *tensors, int64_t n_tensors
   A.log_b2 = beta2 > 0 ? log(beta2) : -1e4;
   A.lr = (float)lr, A.b1 = (float)beta1, A.b2 = (float)beta2;
   A.one_minus_b1 = (float)(1 - beta1), A.one_minus_b2 = (float)(1 - beta2);
-  A.eps = (float)eps, A.wd = (float)weight_decay;
+  A.eps = (float)eps, A.wd = (float)weight_decay, A.one = 1.f;
   A.seed = seed, A.grad_type = grad_type, A.copy_type = copy_type;
 #define SCN_BY_BITS(P) (state_bits == 8 ? launch_list<P, 8>(tensors, n_tensors, A, stream) : launch_list<P, 32>(tensors, n_tensors, A, stream))
   return param_type == SCN_TYPE_FLOAT32 ? SCN_BY_BITS(float) : param_type == SCN_TYPE_BFLOAT16 ? SCN_BY_BITS(__nv_bfloat16) : SCN_BY_BITS(__half);
