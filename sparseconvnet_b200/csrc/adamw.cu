@@ -134,17 +134,11 @@ __device__ __forceinline__ void put(float *p, long long i, float v) { p[i] = v; 
 __device__ __forceinline__ void put(__nv_bfloat16 *p, long long i, float v) { p[i] = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(__half *p, long long i, float v) { p[i] = __float2half_rn(v); }
 
-// 8 values from `at` on (vectors), or the values at + 32 j that lie below n
-template <typename T, bool WHOLE>
+// The values at + 32 j that lie below n; 8 values from `at` on (vectors) where a block is whole
+template <typename T>
 __device__ __forceinline__ void get8(const void *p, long long at, long long n, float (&v)[8]) {
-  if (WHOLE) {
-    unsigned w[Words<T>::N];
-    load_words((const T *)p + at, w);
-    unpack8(w, v, T());
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = at + 32 * j < n ? one<T>(p, at + 32 * j) : 0.f;
-  }
+  for (int j = 0; j < 8; ++j) v[j] = at + 32 * j < n ? one<T>(p, at + 32 * j) : 0.f;
 }
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void put8(void *p, long long at, long long n, const float (&v)[8]) {
@@ -158,19 +152,12 @@ __device__ __forceinline__ void put8(void *p, long long at, long long n, const f
       if (at + 32 * j < n) put((T *)p, at + 32 * j, v[j]);
   }
 }
-template <bool WHOLE>
 __device__ __forceinline__ void get8_e4m3(const void *p, long long at, long long n, float scale, float (&v)[8]) {
   const unsigned char *b = (const unsigned char *)p;
-  uint2 q;
-  if (WHOLE) {
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(b + at));
-  } else {
-    unsigned c[8];
+  unsigned c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = at + 32 * j < n ? b[at + 32 * j] : 0u;
-    q = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-  }
-  from_e4m3(q, scale, v);
+  for (int j = 0; j < 8; ++j) c[j] = at + 32 * j < n ? b[at + 32 * j] : 0u;
+  from_e4m3(make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24), scale, v);
 }
 template <bool WHOLE>
 __device__ __forceinline__ void put8_e4m3(void *p, long long at, long long n, const float (&v)[8]) {
@@ -185,26 +172,78 @@ __device__ __forceinline__ void put8_e4m3(void *p, long long at, long long n, co
   }
 }
 
+// What a warp reads of a block: asked for one block ahead where the block is whole (lane l has values 8 l to 8 l + 7).
+template <typename P, int BITS>
+struct Ahead {
+  unsigned p[Words<P>::N], g[8], m[BITS == 8 ? 2 : 8], v[BITS == 8 ? 2 : 8];
+  float m_scale, v_scale;
+  __device__ __forceinline__ void ask(const Entry &E, const Step &A, long long at, int lane) {
+    const long long first = at * kBlock + lane * 8;
+    load_words((const P *)E.p + first, p);
+    if (A.grad_type == SCN_TYPE_FLOAT32) {
+      load_words((const float *)E.g + first, g);
+    } else {
+      unsigned w[4];
+      load_words((const unsigned short *)E.g + first, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = w[i];
+    }
+    if constexpr (BITS == 8) {
+      load_words((const unsigned char *)E.m + first, m);
+      load_words((const unsigned char *)E.v + first, v);
+      m_scale = __ldg(E.m_scale + at), v_scale = __ldg(E.v_scale + at);
+    } else {
+      load_words((const float *)E.m + first, m);
+      load_words((const float *)E.v + first, v);
+    }
+  }
+  __device__ __forceinline__ void take(const Step &A, float (&pf)[8], float (&gf)[8], float (&mf)[8], float (&rf)[8]) const {
+    unpack8(p, pf, P());
+    if (A.grad_type == SCN_TYPE_FLOAT32) {
+      unpack8(g, gf, 0.f);
+    } else {
+      const unsigned w[4] = {g[0], g[1], g[2], g[3]};
+      if (A.grad_type == SCN_TYPE_BFLOAT16)
+        unpack8(w, gf, __nv_bfloat16());
+      else
+        unpack8(w, gf, __half());
+    }
+    if constexpr (BITS == 8) {
+      from_e4m3(make_uint2(m[0], m[1]), m_scale, mf);
+      from_e4m3(make_uint2(v[0], v[1]), v_scale, rf);
+    } else {
+      unpack8(m, mf, 0.f);
+      unpack8(v, rf, 0.f);
+    }
+  }
+};
+
+// A block that ends early, or whose tensors lie on odd addresses: lane l has values l, l + 32 ..
+template <typename P, int BITS>
+__device__ __forceinline__ void read_block(const Entry &E, const Step &A, long long at, int lane, float (&p)[8], float (&g)[8], float (&m)[8],
+                                           float (&r)[8]) {
+  const long long first = at * kBlock + lane;
+  get8<P>(E.p, first, E.n, p);
+  if (A.grad_type == SCN_TYPE_FLOAT32)
+    get8<float>(E.g, first, E.n, g);
+  else if (A.grad_type == SCN_TYPE_BFLOAT16)
+    get8<__nv_bfloat16>(E.g, first, E.n, g);
+  else
+    get8<__half>(E.g, first, E.n, g);
+  if (BITS == 8) {
+    get8_e4m3(E.m, first, E.n, E.m_scale[at], m);
+    get8_e4m3(E.v, first, E.n, E.v_scale[at], r);
+  } else {
+    get8<float>(E.m, first, E.n, m);
+    get8<float>(E.v, first, E.n, r);
+  }
+}
+
 // One block of 256 values: block `number` of the list, `at` of its tensor
 template <typename P, int BITS, bool WHOLE>
 __device__ __forceinline__ void one_block(const Entry &E, const Step &A, long long at, long long number, unsigned key, float rate,
-                                          float per_root, int lane) {
+                                          float per_root, int lane, float (&p)[8], float (&g)[8], float (&m)[8], float (&r)[8]) {
   const long long first = at * kBlock + (WHOLE ? lane * 8 : lane);
-  float p[8], g[8], m[8], r[8];
-  get8<P, WHOLE>(E.p, first, E.n, p);
-  if (A.grad_type == SCN_TYPE_FLOAT32)
-    get8<float, WHOLE>(E.g, first, E.n, g);
-  else if (A.grad_type == SCN_TYPE_BFLOAT16)
-    get8<__nv_bfloat16, WHOLE>(E.g, first, E.n, g);
-  else
-    get8<__half, WHOLE>(E.g, first, E.n, g);
-  if (BITS == 8) {
-    get8_e4m3<WHOLE>(E.m, first, E.n, E.m_scale[at], m);
-    get8_e4m3<WHOLE>(E.v, first, E.n, E.v_scale[at], r);
-  } else {
-    get8<float, WHOLE>(E.m, first, E.n, m);
-    get8<float, WHOLE>(E.v, first, E.n, r);
-  }
   const Two b1 = two(A.b1), b2 = two(A.b2), c1 = two(A.one_minus_b1), c2 = two(A.one_minus_b2), keep = two(1.f - A.wd);
   // The roundings of the formula as it is written: a sum of products that came out one unit apart would be rounded to the
   // other neighbour now and then.  Pairs' mul.rn and add.rn do get contracted; times one, which the compiler cannot see, not.
@@ -293,14 +332,31 @@ k_adamw(const __grid_constant__ Table<CAP> T, const __grid_constant__ Step A) {
       else
         hi = mid - 1;
     }
-    for (; b < end; b += warps) {
+    long long at;
+    bool whole;
+    Ahead<P, BITS> ahead;
+    auto find = [&] {  // block b's tensor, and what it needs on its way
       while (lo + 1 < A.count && T.e[lo + 1].first >> 1 <= b) ++lo;
       const Entry &E = T.e[lo];
-      const long long at = b - (E.first >> 1);
-      if ((E.first & 1) && (at + 1) * kBlock <= E.n)
-        one_block<P, BITS, true>(E, B, at, b, key, rate, per_root, lane);
-      else
-        one_block<P, BITS, false>(E, B, at, b, key, rate, per_root, lane);
+      at = b - (E.first >> 1);
+      whole = (E.first & 1) && (at + 1) * kBlock <= E.n;
+      if (whole) ahead.ask(E, A, at, lane);
+    };
+    for (find(); b < end;) {
+      const Entry &E = T.e[lo];
+      const long long number = b, mine = at;
+      float p[8], g[8], m[8], r[8];
+      if (whole) {
+        ahead.take(A, p, g, m, r);
+        b += warps;
+        if (b < end) find();
+        one_block<P, BITS, true>(E, B, mine, number, key, rate, per_root, lane, p, g, m, r);
+      } else {
+        read_block<P, BITS>(E, A, mine, lane, p, g, m, r);
+        b += warps;
+        if (b < end) find();
+        one_block<P, BITS, false>(E, B, mine, number, key, rate, per_root, lane, p, g, m, r);
+      }
     }
   }
   if (!A.last) return;

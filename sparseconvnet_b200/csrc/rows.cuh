@@ -61,6 +61,9 @@ __device__ __forceinline__ void load_words(const void *p, unsigned (&w)[8]) {
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                : "l"(p));
 }
+__device__ __forceinline__ void load_words(const void *p, unsigned (&w)[2]) {
+  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+}
 __device__ __forceinline__ void store_words(void *p, const unsigned (&w)[4]) {
   __stcs(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
 }
