@@ -59,7 +59,13 @@ struct GroupParams {
   unsigned idesc;          // without N
   void *out;
   int out_type, vectors, part_vectors;  // vectors_of the results and of the partial sums
-  float *partial;          // weights: [unit of a group of several units][m][n]
+  int m_rows;              // weights: rows of the result with that of the bias sums, if a tile has room for it
+  void *d_bias;
+  int bias_vectors;
+  const float *a, *b;      // fp32 operands that the kernel splits itself
+  long long a_stride, b_stride;
+  int a_quads, b_quads;    // their rows take 16-byte loads
+  float *partial;          // weights: [unit of a group of several units][m_rows][n]
   const void *bias;
   int bias_type;
   const float *row_scale, *col_scale;
@@ -72,7 +78,7 @@ struct Shared {
   unsigned tmem;
   int abort, issued;
   unsigned tails, tail_last;  // stages that have been a sum's end, and the parity of the last time
-  int warp_sums[kThreads / 32];
+  int warp_sums[32];
   __align__(16) float columns[kEpilogueWarps][32];
   int first[kMostGroups + 3];  // units (of rows) before the group
   int begin[kMostGroups + 2], end[kMostGroups + 2];
@@ -320,11 +326,14 @@ __device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, co
     __syncwarp();
   }
   if (WEIGHTS) {
-    if (u.m0 + lane_row >= P.m) return;
-    const bool part = u.part >= 0;
-    const long long row = (part ? (long long)u.part : u.group) * P.m + u.m0 + lane_row;
-    store32(part ? (void *)P.partial : P.out, part ? (int)SCN_TYPE_FLOAT32 : P.out_type, part ? P.part_vectors : P.vectors, row * P.n + c,
-            P.n - c, v);
+    const int m = u.m0 + lane_row;
+    if (m >= P.m_rows) return;
+    if (u.part >= 0)
+      store32(P.partial, SCN_TYPE_FLOAT32, P.part_vectors, ((long long)u.part * P.m_rows + m) * P.n + c, P.n - c, v);
+    else if (m < P.m)
+      store32(P.out, P.out_type, P.vectors, ((long long)u.group * P.m + m) * P.n + c, P.n - c, v);
+    else
+      store32(P.d_bias, P.out_type, P.bias_vectors, (long long)u.group * P.n + c, P.n - c, v);
     return;
   }
   if (lane_row < u.rows) store32(P.out, P.out_type, P.vectors, (long long)(u.row + lane_row) * P.n + c, P.n - c, v);
@@ -798,6 +807,38 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// 8 fp32 values as PARTS times 8 bf16 values: x = h + m + l, each part rounded to nearest of what the ones before leave
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&v)[8], unsigned (&w)[3][4]) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(v[j]) & 0x7FFFFFFFu));
+  if (PARTS == 1 || __float_as_uint(most) < 0x7F7F8000u) {  // (below what rounds to bf16's infinity)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = v[2 * j], b = v[2 * j + 1];
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        w[p][j] = pair(a, b, __nv_bfloat16());
+        a -= __uint_as_float(w[p][j] << 16), b -= __uint_as_float(w[p][j] & 0xFFFF0000u);
+      }
+    }
+    return;
+  }
+  // a value above bf16's largest is cut off instead; an infinity or a NaN has no further parts
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float rest = v[j];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+      if ((b & 0x7FFF) == 0x7F80 && isfinite(rest)) b = __float_as_uint(rest) >> 16;
+      w[p][j / 2] = j % 2 ? w[p][j / 2] | b << 16 : b;
+      rest = isfinite(rest) ? rest - __uint_as_float(b << 16) : 0.f;
+    }
+  }
+}
+
 // Rows of a matrix as `parts` matrices of 16-bit values (or 8-bit ones, copied), planes padded with zeros to whole 16 bytes:
 // what the copies above need where the operand is fp32 or its rows do not lie on 16 bytes.  One thread per 16 bytes of
 // a part.  Bound by HBM: 4 bytes in, 2 per part out.
@@ -822,23 +863,7 @@ k_group_parts(const T *__restrict__ src, long long stride, int planes, long long
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = c + j < planes ? __ldg((const float *)from + j) : 0.f;
     }
-    unsigned short h[3][8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float rest = v[j];
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
-        // (a value above bf16's largest is cut off instead; an infinity or a NaN has no further parts)
-        if (PARTS > 1 && (b & 0x7FFF) == 0x7F80 && isfinite(rest)) b = __float_as_uint(rest) >> 16;
-        h[p][j] = (unsigned short)b;
-        rest = isfinite(rest) ? rest - __uint_as_float(b << 16) : 0.f;
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[p][j] = h[p][2 * j] | (unsigned)h[p][2 * j + 1] << 16;
+    split8<PARTS>(v, w);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -848,6 +873,299 @@ k_group_parts(const T *__restrict__ src, long long stride, int planes, long long
   }
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4 *>(dst + p * part_bytes + i * 16) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// ---- fp32 operands, split on their way --------------------------------------------------------------------------------------
+// The products of fp32 rows for layers of few planes, where a tile is a few steps long and the rows' bytes are what it costs:
+// eight more warps read the fp32 rows, split them and write the parts into the operands' places, so that the parts are never
+// in memory (4 bytes a value in instead of 4 in, 6 out and 6 in again).  A sum is at most kSplitSteps steps long, so that it
+// needs no hand-over between: rows of up to 256 planes, units of 256 rows for the weights' gradient, whose partial sums are
+// added by k_group_sum.  Where the results' rows (planes of x) leave a row of the last tile free, a plane of ones in x makes
+// that row the bias sums.
+constexpr int kSplitSteps = 4, kSplitWarps = 8, kSplitThreads = kThreads + kSplitWarps * 32;
+
+struct Cursor {  // a batch of pieces: the left or the right operand of a step
+  long long i;
+  Unit u;
+  int k, steps, side, step;
+  bool live;
+};
+
+template <int PARTS, int TN, bool WEIGHTS, bool B_ROWS>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupParams P) {
+  SCN_GRID_WAIT();
+  constexpr int kABytes = kTileM * kRow, kBBytes = TN * kRow, kStage = PARTS * (kABytes + kBBytes);
+  constexpr int kStages = kRing / kStage < kMostStages ? kRing / kStage : kMostStages, kAccs = PARTS > 1 ? 2 : 1, kColumns = 256;
+  static_assert(kAccs * TN <= kColumns && kStages >= 2, "shape");
+  extern __shared__ unsigned char raw[];
+  unsigned char *ring = raw + (1024 - smem_u32(raw) % 1024) % 1024;
+  __shared__ Shared S;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  volatile int *abort = &S.abort;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&S.full[i], kSplitWarps + !WEIGHTS), mbar_init(&S.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&S.ready[i], 1), mbar_init(&S.taken[i], kEpilogueWarps);
+    S.abort = 0;
+    S.issued = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(&S.tmem, 512);
+  scan_groups<WEIGHTS>(P, S);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = S.tmem;
+  const int all = WEIGHTS ? P.groups : P.groups + 2;
+  const long long units = (long long)S.first[all] * P.n_tiles * (WEIGHTS ? P.m_tiles : 1);
+  auto steps_of = [&](const Unit &u) { return ((WEIGHTS ? u.rows : u.group < P.groups ? P.k : 0) + kStageRows - 1) / kStageRows; };
+
+  // ==== weights ====
+  if (warp == 0) {
+    const bool lead = elect_one();
+    int step = 0;
+    bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = walk.at(i);
+      const int steps = WEIGHTS ? 0 : steps_of(u);
+      for (int k = 0; k < steps; ++k, ++step) {
+        const int st = step % kStages;
+        if (step >= kStages && !mbar_wait_warp(&S.empty[st], (step / kStages - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        if (lead) {
+          const unsigned b = smem_u32(ring) + st * kStage + PARTS * kABytes;
+          mbar_expect_tx(&S.full[st], PARTS * kBBytes);
+          for (int p = 0; p < PARTS; ++p) {
+            if (B_ROWS)
+              for (int j = 0; j < TN / 64; ++j) load_tile(b + p * kBBytes + j * kStageRows * kRow, &map_b, u.n0 + 64 * j, k * kStageRows, u.group, p, &S.full[st]);
+            else
+              load_tile(b + p * kBBytes, &map_b, k * kStageRows, u.n0, u.group, p, &S.full[st]);
+          }
+          S.issued = step + 1;
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== instructions ====
+  else if (warp == 1) {
+    const unsigned lead = elect_one();
+    int step = 0, turn = 0;
+    bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = walk.at(i);
+      const int steps = steps_of(u);
+      if (!steps) continue;
+      const unsigned idesc = P.idesc | (unsigned)(min(TN, (P.n - u.n0 + 15) / 16 * 16) >> 3) << 17;
+      if (turn >= 2 && !mbar_wait_warp(&S.taken[turn & 1], ((turn >> 1) - 1) & 1, abort)) ok = false;
+      for (int k = 0; k < steps && ok; ++k, ++step) {
+        const int st = step % kStages;
+        if (!mbar_wait_warp(&S.full[st], (step / kStages) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const unsigned a = smem_u32(ring) + st * kStage, b = a + PARTS * kABytes, d = tmem + (turn & 1) * kColumns;
+        const int instructions = ((WEIGHTS ? min(kStageRows, u.rows - k * kStageRows) : min(kStageRows, P.k - k * kStageRows)) + 15) / 16;
+        for (int j = 0; j < instructions; ++j) {
+#pragma unroll
+          for (int q = 0; q < Products<PARTS>::N; ++q) {
+            const unsigned pa = a + part_a(q) * kABytes + j * (WEIGHTS ? 16 * kRow : 32), pb = b + part_b(q) * kBBytes + j * (WEIGHTS || B_ROWS ? 16 * kRow : 32);
+            const unsigned fresh = k == 0 && j == 0 && (q == 0 || q == 1);
+            mma_if<false>(lead, d + (q ? TN : 0), desc_lo(pa, WEIGHTS ? kStageRows * kRow : 16), kDescHi, desc_lo(pb, WEIGHTS || B_ROWS ? kStageRows * kRow : 16),
+                          kDescHi, idesc, !fresh);
+          }
+        }
+        if (!(P.drop && blockIdx.x == 0 && step == 0)) tc_commit_if(lead, &S.empty[st]);
+        if (k == steps - 1) tc_commit_if(lead, &S.ready[turn & 1]);
+        __syncwarp();
+      }
+      ++turn;
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== results ====
+  else if (warp < 2 + kEpilogueWarps) {
+    const int quarter = warp % 4, half = (warp - 2) / 4;
+    constexpr int kMine = TN / 2;
+    const int lane_row = quarter * 32 + lane;
+    int turn = 0;
+    bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
+    for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = walk.at(i);
+      const int columns = min(P.n - u.n0 - half * kMine, kMine);
+      const bool summed = steps_of(u) > 0;
+      Terms<kMine, WEIGHTS, false> terms;
+      terms.read(P, u, u.n0 + half * kMine, lane_row, lane);
+      if (summed && !mbar_wait_warp(&S.ready[turn & 1], (turn >> 1) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const unsigned from = tmem + ((unsigned)(quarter * 32) << 16) + (turn & 1) * kColumns + half * kMine;
+#pragma unroll
+      for (int c = 0; c < kMine; c += 32) {
+        if (c >= columns) break;
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        if (summed) {
+          tmem_ld32(from + c, v);
+          if (kAccs == 2) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              float low[16];
+              tmem_ld16(from + TN + c + e, low);
+#pragma unroll
+              for (int f = 0; f < 16; ++f) v[e + f] += low[f];
+            }
+          }
+        }
+        finish32(P, u, terms, c / 32, lane_row, u.n0 + half * kMine + c, S.columns[warp - 2], v);
+      }
+      if (summed) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.taken[turn & 1]);
+        ++turn;
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  // ==== rows ====
+  else {
+    const int t = tid - kThreads;  // 0 .. 255
+    bool ok = true;
+    Walk<WEIGHTS, TN> walk(P, S);
+    Cursor next;
+    next.i = blockIdx.x, next.k = next.side = next.step = 0;
+    auto settle = [&] {  // on to a unit that has steps
+      for (next.live = false; next.i < units; next.i += gridDim.x) {
+        next.u = walk.at(next.i);
+        next.steps = steps_of(next.u);
+        if (next.steps) {
+          next.live = true;
+          break;
+        }
+      }
+    };
+    auto advance = [&] {
+      if (WEIGHTS && next.side == 0) {
+        next.side = 1;
+        return;
+      }
+      next.side = 0;
+      ++next.step;
+      if (++next.k < next.steps) return;
+      next.k = 0;
+      next.i += gridDim.x;
+      settle();
+    };
+    // A piece: 8 values, 16 bytes of each part.  Left: 4 pieces a thread; right: TN / 32 (weights' gradient only).
+    constexpr int kRight = TN / 32;
+    auto place_of = [&](const Cursor &c, int i, int &row, int &chunk) {
+      const int wide = WEIGHTS && (c.side == 0 || TN == 128) ? 16 : 8;  // pieces of a row
+      row = (i * 256 + t) / wide, chunk = t % wide;
+    };
+    auto fetch = [&](const Cursor &c, float (&v)[4][8]) {
+      const bool left = c.side == 0;
+      const float *from = left ? P.a : P.b;
+      const long long stride = left ? P.a_stride : P.b_stride;
+      const int limit = !WEIGHTS ? P.k : left ? P.m : P.n, col0 = !WEIGHTS ? c.k * kStageRows : left ? c.u.m0 : c.u.n0;
+      const int rows = WEIGHTS ? c.u.rows - c.k * kStageRows : c.u.rows, first = c.u.row + (WEIGHTS ? c.k * kStageRows : 0);
+      const bool quads = left ? P.a_quads : P.b_quads;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= kRight && !left) break;
+        int row, chunk;
+        place_of(c, i, row, chunk);
+        const int col = col0 + chunk * 8;
+        const float *p = from + (first + row) * stride + col;
+        const bool in = row < rows;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (quads) {
+            if (in && col + j < limit) q = __ldg((const float4 *)(p + j));
+          } else if (in) {
+            if (col + j < limit) q.x = __ldg(p + j);
+            if (col + j + 1 < limit) q.y = __ldg(p + j + 1);
+            if (col + j + 2 < limit) q.z = __ldg(p + j + 2);
+            if (col + j + 3 < limit) q.w = __ldg(p + j + 3);
+          }
+          v[i][j] = q.x, v[i][j + 1] = q.y, v[i][j + 2] = q.z, v[i][j + 3] = q.w;
+        }
+      }
+    };
+    auto put = [&](const Cursor &c, float (&v)[4][8]) {
+      const bool left = c.side == 0;
+      const int col0 = !WEIGHTS ? 0 : left ? c.u.m0 : c.u.n0, limit = !WEIGHTS ? 0 : left ? P.m_rows : P.n;
+      const int rows = WEIGHTS ? c.u.rows - c.k * kStageRows : c.u.rows;
+      unsigned char *to = ring + c.step % kStages * kStage + (left ? 0 : PARTS * kABytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= kRight && !left) break;
+        int row, chunk;
+        place_of(c, i, row, chunk);
+        const int col = col0 + chunk * 8;
+        // Rows and planes that no result needs keep what is there.  Rows behind a sum's last are needed, as zeros.
+        if (WEIGHTS ? col >= limit : row >= rows) continue;
+        if (WEIGHTS && left && P.d_bias && P.m_rows > P.m) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (col + j == P.m) v[i][j] = row < rows ? 1.f : 0.f;
+        }
+        unsigned w[3][4];
+        split8<PARTS>(v[i], w);
+        unsigned char *at = to + (WEIGHTS ? chunk / 8 * (kStageRows * kRow) : 0) + row * kRow + ((chunk % 8) ^ (row & 7)) * 16;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+          *reinterpret_cast<uint4 *>(at + p * (left ? kABytes : kBBytes)) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+      }
+    };
+    settle();
+    float v[4][8];
+    if (next.live) fetch(next, v);
+    while (next.live) {
+      const Cursor c = next;
+      float now[4][8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) now[i][j] = v[i][j];
+      advance();
+      if (next.live) fetch(next, v);
+      const int st = c.step % kStages;
+      if (c.side == 0 && c.step >= kStages && !mbar_wait_warp(&S.empty[st], (c.step / kStages - 1) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      put(c, now);
+      if (!WEIGHTS || c.side == 1) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.full[st]);
+      }
+    }
+    if (!ok && lane == 0) *abort = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (S.abort && tid == 0) {  // the weights' copies land before the block ends
+    atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+    // (a stage's barrier also counts the rows, which may not come any more: a bounded wait is long enough for a copy to land)
+    for (int s = 0; s < kStages; ++s)
+      if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 __device__ __forceinline__ void put_value(void *out, int type, long long at, float v) {
@@ -865,7 +1183,7 @@ k_group_sum(const __grid_constant__ GroupParams P) {
   SCN_GRID_WAIT();
   __shared__ Shared S;
   scan_groups<true>(P, S);
-  const long long size = (long long)P.m * P.n;
+  const long long size = (long long)P.m_rows * P.n, weights = (long long)P.m * P.n;
   for (int g = blockIdx.y; g < P.groups; g += gridDim.y) {
     if (S.part[g] < 0) continue;
     const int units = S.first[g + 1] - S.first[g];
@@ -881,7 +1199,10 @@ k_group_sum(const __grid_constant__ GroupParams P) {
         for (int j = 0; j < 8; ++j) v += x[j];
       }
       for (; u < units; ++u) v += __ldg(from + u * size + i);
-      put_value(P.out, P.out_type, g * size + i, v);
+      if (i < weights)
+        put_value(P.out, P.out_type, g * weights + i, v);
+      else
+        put_value(P.d_bias, P.out_type, (long long)g * P.n + i - weights, v);
     }
   }
 }
@@ -1128,7 +1449,7 @@ int chunk_of(long long n_rows, long long tiles) {
 }
 
 int sum_parts(GroupParams P, cudaStream_t stream) {
-  const long long size = (long long)P.m * P.n;
+  const long long size = (long long)P.m_rows * P.n;
   const long long across = std::min<long long>(ceil_div(size, 256), 4 * kSms), groups = std::min<long long>(P.groups, ceil_div(8 * kSms, across));
   SCN_LAUNCH(k_group_sum, dim3((unsigned)across, (unsigned)groups), 256, 0, stream, P);
   SCN_CUDA_CHECK(cudaGetLastError());
@@ -1146,7 +1467,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
   P.tile = pair ? 2 * kTileM : kTileM;
-  P.m = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
+  P.m = P.m_rows = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
   P.idesc = idesc_of(type, true, true, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
@@ -1167,10 +1488,80 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   return split ? sum_parts(P, stream) : SCN_OK;
 }
 
+template <int PARTS, int TN, bool WEIGHTS, bool B_ROWS>
+int launch_split(const CUtensorMap &b, const GroupParams &P, long long most_units, cudaStream_t stream) {
+  constexpr size_t smem = kRing + 1024;
+  static std::atomic<int> known[64];
+  int dev = 0;
+  SCN_CUDA_CHECK(cudaGetDevice(&dev));
+  SCN_REQUIRE(dev >= 0 && dev < 64, SCN_ERR_UNSUPPORTED, "device index %d unsupported", dev);
+  constexpr auto kernel = k_group_split<PARTS, TN, WEIGHTS, B_ROWS>;
+  int blocks = known[dev].load();
+  if (!blocks) {
+    SCN_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    SCN_CUDA_CHECK(cudaDeviceGetAttribute(&blocks, cudaDevAttrMultiProcessorCount, dev));
+    known[dev].store(blocks);
+  }
+  SCN_LAUNCH(kernel, (unsigned)std::min<long long>(blocks, most_units), kSplitThreads, smem, stream, b, P);
+  SCN_CUDA_CHECK(cudaGetLastError());
+  return SCN_OK;
+}
+
+int quads_of(const void *p, long long stride, int planes) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0 && planes % 4 == 0; }
+
+// rows_product of fp32 rows, split in the kernel: sums of at most kSplitSteps steps
+bool splits_rows(int type, int k) { return type == SCN_TYPE_FLOAT32 && k <= kSplitSteps * kStageRows; }
+int rows_product_split(const Groups &G, const void *x, long long stride, const Operand &w, bool b_rows, int parts, int k, int n, void *out,
+                       int out_type, const void *bias, int bias_type, int drop, cudaStream_t stream) {
+  const long long row_tiles = G.n_rows / kTileM + std::min<long long>(G.groups + 2, G.n_rows);
+  const int tn = tile_columns(row_tiles, n, 128);
+  GroupParams P{};
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.tile = kTileM;
+  P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
+  P.idesc = idesc_of(SCN_TYPE_BFLOAT16, false, b_rows, kTileM);
+  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_type == SCN_TYPE_FLOAT32 ? 4 : 2);
+  P.bias = bias, P.bias_type = bias_type, P.drop = drop;
+  P.a = (const float *)x, P.a_stride = stride, P.a_quads = quads_of(x, stride, k);
+  CUtensorMap b;
+  SCN_TRY(b_rows ? make_map(&b, w, SCN_TYPE_BFLOAT16, n, k, G.groups, parts, 64, 64) : make_map(&b, w, SCN_TYPE_BFLOAT16, k, n, G.groups, parts, 64, tn));
+  const long long most = row_tiles * P.n_tiles;
+#define SCN_TN(PARTS, B_ROWS) (tn == 64 ? launch_split<PARTS, 64, false, B_ROWS>(b, P, most, stream) : launch_split<PARTS, 128, false, B_ROWS>(b, P, most, stream))
+#define SCN_MAJOR(PARTS) (b_rows ? SCN_TN(PARTS, true) : SCN_TN(PARTS, false))
+  return parts == 1 ? SCN_MAJOR(1) : parts == 2 ? SCN_MAJOR(2) : SCN_MAJOR(3);
+#undef SCN_MAJOR
+#undef SCN_TN
+}
+
+// weights_product of fp32 rows, split in the kernel, with the bias sums where they fit (*bias_done).  Its units are short, so
+// the partial sums have to be small beside the rows: 256 rows of m + n values against m n sums.
+bool splits_weights(int type, int m, int n) { return type == SCN_TYPE_FLOAT32 && m <= 128 && n <= 256; }
+int weights_product_split(const Groups &G, const void *x, long long x_stride, const void *dy, long long dy_stride, int m, int n, void *out,
+                          void *d_bias, bool *bias_done, Scratch &scratch, cudaStream_t stream) {
+  const int tn = n <= 64 ? 64 : 128;
+  GroupParams P{};
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.tile = kTileM;
+  *bias_done = d_bias && m % kTileM != 0;
+  P.m = m, P.m_rows = m + *bias_done, P.n = n, P.m_tiles = (int)ceil_div(m, kTileM), P.n_tiles = (int)ceil_div(n, tn);
+  P.chunk = kSplitSteps * kStageRows;
+  P.idesc = idesc_of(SCN_TYPE_BFLOAT16, true, true, kTileM);
+  P.out = out, P.out_type = SCN_TYPE_FLOAT32, P.vectors = vectors_of((uintptr_t)out, n, 4), P.part_vectors = vectors_of(0, n, 4);
+  P.d_bias = *bias_done ? d_bias : nullptr, P.bias_vectors = vectors_of((uintptr_t)d_bias, n, 4);
+  P.a = (const float *)x, P.a_stride = x_stride, P.a_quads = quads_of(x, x_stride, m);
+  P.b = (const float *)dy, P.b_stride = dy_stride, P.b_quads = quads_of(dy, dy_stride, n);
+  const bool split = G.n_rows > P.chunk;
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * P.m_rows * n));
+  const long long most = (ceil_div(G.n_rows, P.chunk) + G.groups) * P.m_tiles * P.n_tiles;
+  const CUtensorMap none{};
+  SCN_TRY((tn == 64 ? launch_split<3, 64, true, true>(none, P, most, stream) : launch_split<3, 128, true, true>(none, P, most, stream)));
+  return split ? sum_parts(P, stream) : SCN_OK;
+}
+
 int bias_sums(const Groups &G, const void *dy, long long stride, int type, int n, void *out, int out_type, Scratch &scratch, cudaStream_t stream) {
   GroupParams P{};
   P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
-  P.m = 1, P.n = n, P.m_tiles = P.n_tiles = 1;
+  P.m = P.m_rows = 1, P.n = n, P.m_tiles = P.n_tiles = 1;
   P.chunk = chunk_of(G.n_rows, std::max<long long>(1, ceil_div(n, 32) / 4));
   P.out = out, P.out_type = out_type;
   const bool split = G.n_rows > P.chunk;
@@ -1216,13 +1607,14 @@ int scn_grouped_product_forward(const void *x, int64_t x_stride, int type, const
   SCN_REQUIRE(x && weight && out, SCN_ERR_BAD_ARG, "grouped_product: null argument");
   const Groups G{offsets, offsets_64, n_rows, n_groups};
   const int parts = parts_of(type, precision), held = type == SCN_TYPE_FLOAT32 ? SCN_TYPE_BFLOAT16 : type;
-  Scratch scratch(stream);
-  Operand a, b;
-  SCN_TRY(operand(x, x_stride, n_in, n_rows, type, parts, scratch, stream, &a));
-  SCN_TRY(operand(weight, n_out, n_out, (long long)n_groups * n_in, type, parts, scratch, stream, &b));
-  b.matrix = b.stride * n_in;
   const int drop = g_drop_arrival;
   g_drop_arrival = 0;
+  Scratch scratch(stream);
+  Operand a, b;
+  SCN_TRY(operand(weight, n_out, n_out, (long long)n_groups * n_in, type, parts, scratch, stream, &b));
+  b.matrix = b.stride * n_in;
+  if (splits_rows(type, n_in)) return rows_product_split(G, x, x_stride, b, true, parts, n_in, n_out, out, out_type, bias, bias_type, drop, stream);
+  SCN_TRY(operand(x, x_stride, n_in, n_rows, type, parts, scratch, stream, &a));
   return rows_product(G, a, b, true, parts, held, n_in, n_out, out, out_type, bias, bias_type, nullptr, nullptr, drop, stream);
 }
 
@@ -1245,20 +1637,26 @@ int scn_grouped_product_backward(const void *x, int64_t x_stride, int type, cons
   // the input's gradient at the precision asked for, the weights' always as fp32
   const int dx_parts = parts_of(type, precision), dw_parts = parts_of(type, SCN_PRECISION_FP32);
   Scratch scratch(stream);
+  const bool split_x = d_x && splits_rows(type, n_out), split_w = d_weight && splits_weights(type, n_in, n_out);
   Operand dy;
-  if (d_x || d_weight) SCN_TRY(operand(d_out, d_out_stride, n_out, n_rows, type, d_weight ? dw_parts : dx_parts, scratch, stream, &dy));
+  if ((d_x && !split_x) || (d_weight && !split_w))
+    SCN_TRY(operand(d_out, d_out_stride, n_out, n_rows, type, d_weight && !split_w ? dw_parts : dx_parts, scratch, stream, &dy));
   if (d_x) {
     Operand w;
     SCN_TRY(operand(weight, n_out, n_out, (long long)n_groups * n_in, type, dx_parts, scratch, stream, &w));
     w.matrix = w.stride * n_in;
-    SCN_TRY(rows_product(G, dy, w, false, dx_parts, held, n_out, n_in, d_x, type, nullptr, 0, nullptr, nullptr, 0, stream));
+    SCN_TRY(split_x ? rows_product_split(G, d_out, d_out_stride, w, false, dx_parts, n_out, n_in, d_x, type, nullptr, 0, 0, stream)
+                    : rows_product(G, dy, w, false, dx_parts, held, n_out, n_in, d_x, type, nullptr, 0, nullptr, nullptr, 0, stream));
   }
-  if (d_weight) {
+  bool bias_done = false;
+  if (split_w) {
+    SCN_TRY(weights_product_split(G, x, x_stride, d_out, d_out_stride, n_in, n_out, d_weight, d_bias, &bias_done, scratch, stream));
+  } else if (d_weight) {
     Operand a;
     SCN_TRY(operand(x, x_stride, n_in, n_rows, type, dw_parts, scratch, stream, &a));
     SCN_TRY(weights_product(G, a, dy, dw_parts, held, n_in, n_out, d_weight, type, scratch, stream));
   }
-  return d_bias ? bias_sums(G, d_out, d_out_stride, type, n_out, d_bias, type, scratch, stream) : SCN_OK;
+  return d_bias && !bias_done ? bias_sums(G, d_out, d_out_stride, type, n_out, d_bias, type, scratch, stream) : SCN_OK;
 }
 
 int scn_grouped_product_quantized(const void *q, int64_t q_stride, const float *scale, const void *weight, const float *weight_scale,

@@ -64,7 +64,9 @@ SHAPES = [([1], 0, 0, 1, 1), ([1, 0, 2], 0, 0, 16, 16), ([5], 3, 2, 8, 24), ([12
           ([3] * 100, 0, 0, 48, 40), ([4000], 0, 0, 40, 64),
           # tiles of two blocks: groups that end in the first and in the second block's rows, inside and at the end of a stage
           ([3000, 0, 5000, 2900], 5, 3, 264, 300), ([2560, 2816, 4096, 1024], 0, 0, 512, 256), ([10001, 77, 1, 640], 0, 0, 136, 1000),
-          ([9000, 130], 1, 1, 1000, 264)]
+          ([9000, 130], 1, 1, 1000, 264),
+          # fp32 rows split in the kernel: up to 256 planes, weights' gradients of up to 128 x 256, with and without room for the bias
+          ([700, 0, 257, 256, 1], 3, 2, 128, 256), ([1, 15, 16, 17, 255, 300], 2, 0, 127, 200), ([500, 40], 0, 1, 257, 100), ([600, 70], 0, 0, 100, 260)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -339,9 +341,10 @@ def test_refusals(cuda):
 def test_a_wait_that_runs_out_is_reported(cuda):
     """Leaves out one arrival in one block: the call gives up in bounded time, poll_errors says so, the next call is right."""
     from sparseconvnet_b200._lib import lib
-    for rows, n in ((256, 256), (20000, 512)):  # one block to a tile, two
+    # one block to a tile, two, and fp32 rows that the kernel splits
+    for rows, k, n, t in ((256, 4096, 256, torch.bfloat16), (20000, 4096, 512, torch.bfloat16), (200000, 256, 64, torch.float32)):
         o = offsets_of([rows])
-        x, w = normal(rows, 4096, t=torch.bfloat16, seed=1), normal(1, 4096, n, t=torch.bfloat16, seed=2)
+        x, w = normal(rows, k, t=t, seed=1), normal(1, k, n, t=t, seed=2)
         want = scn.grouped_product(x, w, o)
         scn.poll_errors()
         lib.scn_test_drop_barrier_arrival()
