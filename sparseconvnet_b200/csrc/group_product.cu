@@ -807,13 +807,11 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// 8 fp32 values as PARTS times 8 bf16 values: x = h + m + l, each part rounded to nearest of what the ones before leave
+// 8 fp32 values as PARTS times 8 bf16 values: x = h + m + l, each part rounded to nearest of what the ones before leave.
+// `plain`: no value is above bf16's largest (it would round to an infinity).
 template <int PARTS>
-__device__ __forceinline__ void split8(const float (&v)[8], unsigned (&w)[3][4]) {
-  float most = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(v[j]) & 0x7FFFFFFFu));
-  if (PARTS == 1 || __float_as_uint(most) < 0x7F7F8000u) {  // (below what rounds to bf16's infinity)
+__device__ __forceinline__ void split8(const float (&v)[8], bool plain, unsigned (&w)[3][4]) {
+  if (plain) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float a = v[2 * j], b = v[2 * j + 1];
@@ -823,20 +821,25 @@ __device__ __forceinline__ void split8(const float (&v)[8], unsigned (&w)[3][4])
         a -= __uint_as_float(w[p][j] << 16), b -= __uint_as_float(w[p][j] & 0xFFFF0000u);
       }
     }
-    return;
-  }
-  // a value above bf16's largest is cut off instead; an infinity or a NaN has no further parts
+  } else {  // such a value is cut off instead; an infinity or a NaN has no further parts
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float rest = v[j];
+    for (int j = 0; j < 8; ++j) {
+      float rest = v[j];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
-      if ((b & 0x7FFF) == 0x7F80 && isfinite(rest)) b = __float_as_uint(rest) >> 16;
-      w[p][j / 2] = j % 2 ? w[p][j / 2] | b << 16 : b;
-      rest = isfinite(rest) ? rest - __uint_as_float(b << 16) : 0.f;
+      for (int p = 0; p < PARTS; ++p) {
+        unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+        if (PARTS > 1 && (b & 0x7FFF) == 0x7F80 && isfinite(rest)) b = __float_as_uint(rest) >> 16;
+        w[p][j / 2] = j % 2 ? w[p][j / 2] | b << 16 : b;
+        rest = isfinite(rest) ? rest - __uint_as_float(b << 16) : 0.f;
+      }
     }
   }
+}
+__device__ __forceinline__ bool all_plain(const float (&v)[8]) {  // (a NaN may take either way: all its parts are NaN)
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+  return __float_as_uint(most) < 0x7F7F8000u;
 }
 
 // Rows of a matrix as `parts` matrices of 16-bit values (or 8-bit ones, copied), planes padded with zeros to whole 16 bytes:
@@ -863,7 +866,7 @@ k_group_parts(const T *__restrict__ src, long long stride, int planes, long long
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = c + j < planes ? __ldg((const float *)from + j) : 0.f;
     }
-    split8<PARTS>(v, w);
+    split8<PARTS>(v, PARTS == 1 || all_plain(v), w);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -877,19 +880,82 @@ k_group_parts(const T *__restrict__ src, long long stride, int planes, long long
 
 // ---- fp32 operands, split on their way --------------------------------------------------------------------------------------
 // The products of fp32 rows for layers of few planes, where a tile is a few steps long and the rows' bytes are what it costs:
-// eight more warps read the fp32 rows, split them and write the parts into the operands' places, so that the parts are never
+// sixteen more warps read the fp32 rows, split them and write the parts into the operands' places, so that the parts are never
 // in memory (4 bytes a value in instead of 4 in, 6 out and 6 in again).  A sum is at most kSplitSteps steps long, so that it
 // needs no hand-over between: rows of up to 256 planes, units of 256 rows for the weights' gradient, whose partial sums are
 // added by k_group_sum.  Where the results' rows (planes of x) leave a row of the last tile free, a plane of ones in x makes
 // that row the bias sums.
-constexpr int kSplitSteps = 4, kSplitWarps = 8, kSplitThreads = kThreads + kSplitWarps * 32;
+constexpr int kSplitSteps = 4, kSplitWarps = 16, kSplitLoaders = kSplitWarps * 32, kSplitThreads = kThreads + kSplitWarps * 32;
 
-struct Cursor {  // a batch of pieces: the left or the right operand of a step
+struct Cursor {  // a step of a unit
   long long i;
   Unit u;
-  int k, steps, side, step;
+  int k, steps, step;
   bool live;
 };
+
+// PIECES pieces (8 values, 16 bytes of each part) of an operand's step, one thread's share: rows of WIDE pieces
+struct Side {
+  const float *p;
+  long long stride;
+  int quads, limit, col0, rows, first;  // limit: planes; rows: below it rows are real; first: the step's first row
+};
+template <int WIDE, int PIECES>
+__device__ __forceinline__ void fetch(const Side &S, int t, float (&v)[PIECES][8]) {
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int row = (i * kSplitLoaders + t) / WIDE, col = S.col0 + t % WIDE * 8;
+    const float *p = S.p + (S.first + row) * S.stride + col;
+    const bool in = row < S.rows;
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (S.quads) {
+        if (in && col + j < S.limit) q = __ldg((const float4 *)(p + j));
+      } else if (in) {
+        if (col + j < S.limit) q.x = __ldg(p + j);
+        if (col + j + 1 < S.limit) q.y = __ldg(p + j + 1);
+        if (col + j + 2 < S.limit) q.z = __ldg(p + j + 2);
+        if (col + j + 3 < S.limit) q.w = __ldg(p + j + 3);
+      }
+      v[i][j] = q.x, v[i][j + 1] = q.y, v[i][j + 2] = q.z, v[i][j + 3] = q.w;
+    }
+  }
+}
+// `ones`: the plane that is one in every real row, -1: none.  Rows (K-major) or planes (M- / N-major) that no result needs keep
+// what is there; rows behind a sum's last are needed, as zeros.
+template <int PARTS, int WIDE, int PIECES, bool K_MAJOR>
+__device__ __forceinline__ void put(const Side &S, int t, int limit, int ones, unsigned char *to, int part_bytes, float (&v)[PIECES][8]) {
+  const int chunk = t % WIDE, col = S.col0 + chunk * 8;
+  bool plain = true;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    if (!K_MAJOR && ones >= 0 && (ones >> 3) == (col >> 3)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j == ones) v[i][j] = (i * kSplitLoaders + t) / WIDE < S.rows ? 1.f : 0.f;
+    }
+    plain = plain && (PARTS == 1 || all_plain(v[i]));
+  }
+  if (!K_MAJOR && col >= limit) return;
+  auto pieces = [&](bool quick) {  // (one branch for all: their chains of roundings and differences overlap)
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int row = (i * kSplitLoaders + t) / WIDE;
+      unsigned w[3][4];
+      split8<PARTS>(v[i], quick, w);
+      unsigned char *at = to + (K_MAJOR ? 0 : chunk / 8 * (kStageRows * kRow)) + row * kRow + ((chunk % 8) ^ (row & 7)) * 16;
+      if (!K_MAJOR || row < S.rows) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4 *>(at + p * part_bytes) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+      }
+    }
+  };
+  if (plain)
+    pieces(true);
+  else
+    pieces(false);
+}
 
 template <int PARTS, int TN, bool WEIGHTS, bool B_ROWS>
 __global__ void __launch_bounds__(kSplitThreads, 1)
@@ -925,6 +991,11 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
     const bool lead = elect_one();
     int step = 0;
     bool ok = true;
+    // what a stage's place for weights holds: tiles of the same group and columns come one after the other, and with no more
+    // steps than stages each finds its slice where the last one left it
+    int held[kStages][3];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) held[i][0] = held[i][1] = held[i][2] = -1;
     Walk<WEIGHTS, TN> walk(P, S);
     for (long long i = blockIdx.x; i < units && ok; i += gridDim.x) {
       const Unit u = walk.at(i);
@@ -935,7 +1006,16 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
           ok = false;
           break;
         }
-        if (lead) {
+        bool here = false;
+#pragma unroll
+        for (int i = 0; i < kStages; ++i)
+          if (i == st) {
+            here = held[i][0] == u.group && held[i][1] == u.n0 && held[i][2] == k;
+            held[i][0] = u.group, held[i][1] = u.n0, held[i][2] = k;
+          }
+        if (here) {
+          if (lead) mbar_arrive(&S.full[st]);
+        } else if (lead) {
           const unsigned b = smem_u32(ring) + st * kStage + PARTS * kABytes;
           mbar_expect_tx(&S.full[st], PARTS * kBBytes);
           for (int p = 0; p < PARTS; ++p) {
@@ -1040,11 +1120,12 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
   }
   // ==== rows ====
   else {
-    const int t = tid - kThreads;  // 0 .. 255
+    const int t = tid - kThreads;
+    constexpr int kLeft = kTileM * 8 / kSplitLoaders, kRight = TN * 8 / kSplitLoaders, kRightWide = TN / 8;  // pieces of a thread
     bool ok = true;
     Walk<WEIGHTS, TN> walk(P, S);
     Cursor next;
-    next.i = blockIdx.x, next.k = next.side = next.step = 0;
+    next.i = blockIdx.x, next.k = next.step = 0;
     auto settle = [&] {  // on to a unit that has steps
       for (next.live = false; next.i < units; next.i += gridDim.x) {
         next.u = walk.at(next.i);
@@ -1056,102 +1137,50 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
       }
     };
     auto advance = [&] {
-      if (WEIGHTS && next.side == 0) {
-        next.side = 1;
-        return;
-      }
-      next.side = 0;
       ++next.step;
       if (++next.k < next.steps) return;
       next.k = 0;
       next.i += gridDim.x;
       settle();
     };
-    // A piece: 8 values, 16 bytes of each part.  Left: 4 pieces a thread; right: TN / 32 (weights' gradient only).
-    constexpr int kRight = TN / 32;
-    auto place_of = [&](const Cursor &c, int i, int &row, int &chunk) {
-      const int wide = WEIGHTS && (c.side == 0 || TN == 128) ? 16 : 8;  // pieces of a row
-      row = (i * 256 + t) / wide, chunk = t % wide;
+    auto left = [&](const Cursor &c) {
+      return WEIGHTS ? Side{P.a, P.a_stride, P.a_quads, P.m, c.u.m0, c.u.rows - c.k * kStageRows, c.u.row + c.k * kStageRows}
+                     : Side{P.a, P.a_stride, P.a_quads, P.k, c.k * kStageRows, c.u.rows, c.u.row};
     };
-    auto fetch = [&](const Cursor &c, float (&v)[4][8]) {
-      const bool left = c.side == 0;
-      const float *from = left ? P.a : P.b;
-      const long long stride = left ? P.a_stride : P.b_stride;
-      const int limit = !WEIGHTS ? P.k : left ? P.m : P.n, col0 = !WEIGHTS ? c.k * kStageRows : left ? c.u.m0 : c.u.n0;
-      const int rows = WEIGHTS ? c.u.rows - c.k * kStageRows : c.u.rows, first = c.u.row + (WEIGHTS ? c.k * kStageRows : 0);
-      const bool quads = left ? P.a_quads : P.b_quads;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i >= kRight && !left) break;
-        int row, chunk;
-        place_of(c, i, row, chunk);
-        const int col = col0 + chunk * 8;
-        const float *p = from + (first + row) * stride + col;
-        const bool in = row < rows;
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (quads) {
-            if (in && col + j < limit) q = __ldg((const float4 *)(p + j));
-          } else if (in) {
-            if (col + j < limit) q.x = __ldg(p + j);
-            if (col + j + 1 < limit) q.y = __ldg(p + j + 1);
-            if (col + j + 2 < limit) q.z = __ldg(p + j + 2);
-            if (col + j + 3 < limit) q.w = __ldg(p + j + 3);
-          }
-          v[i][j] = q.x, v[i][j + 1] = q.y, v[i][j + 2] = q.z, v[i][j + 3] = q.w;
-        }
+    auto right = [&](const Cursor &c) { return Side{P.b, P.b_stride, P.b_quads, P.n, c.u.n0, c.u.rows - c.k * kStageRows, c.u.row + c.k * kStageRows}; };
+    // The next step's values are on their way while the present one's are split: rows by two sets of registers in turn, for the
+    // weights' gradient the left operand's while the right one's are split and the other way round.
+    float va[kLeft][8], vb[WEIGHTS ? kRight : kLeft][8];
+    auto one = [&](auto &now, auto &then) {
+      const Cursor c = next;
+      unsigned char *to = ring + c.step % kStages * kStage;
+      if constexpr (!WEIGHTS) {
+        advance();
+        if (next.live) fetch<8, kLeft>(left(next), t, then);
       }
-    };
-    auto put = [&](const Cursor &c, float (&v)[4][8]) {
-      const bool left = c.side == 0;
-      const int col0 = !WEIGHTS ? 0 : left ? c.u.m0 : c.u.n0, limit = !WEIGHTS ? 0 : left ? P.m_rows : P.n;
-      const int rows = WEIGHTS ? c.u.rows - c.k * kStageRows : c.u.rows;
-      unsigned char *to = ring + c.step % kStages * kStage + (left ? 0 : PARTS * kABytes);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i >= kRight && !left) break;
-        int row, chunk;
-        place_of(c, i, row, chunk);
-        const int col = col0 + chunk * 8;
-        // Rows and planes that no result needs keep what is there.  Rows behind a sum's last are needed, as zeros.
-        if (WEIGHTS ? col >= limit : row >= rows) continue;
-        if (WEIGHTS && left && P.d_bias && P.m_rows > P.m) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (col + j == P.m) v[i][j] = row < rows ? 1.f : 0.f;
-        }
-        unsigned w[3][4];
-        split8<PARTS>(v[i], w);
-        unsigned char *at = to + (WEIGHTS ? chunk / 8 * (kStageRows * kRow) : 0) + row * kRow + ((chunk % 8) ^ (row & 7)) * 16;
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-          *reinterpret_cast<uint4 *>(at + p * (left ? kABytes : kBBytes)) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+      if (c.step >= kStages && !mbar_wait_warp(&S.empty[c.step % kStages], (c.step / kStages - 1) & 1, abort)) return false;
+      if constexpr (!WEIGHTS) {
+        put<PARTS, 8, kLeft, true>(left(c), t, 0, -1, to, kABytes, now);
+      } else {
+        put<PARTS, 16, kLeft, false>(left(c), t, P.m_rows, P.m_rows > P.m ? P.m : -1, to, kABytes, va);
+        advance();
+        if (next.live) fetch<16, kLeft>(left(next), t, va);
+        put<PARTS, kRightWide, kRight, false>(right(c), t, P.n, -1, to + PARTS * kABytes, kBBytes, vb);
+        if (next.live) fetch<kRightWide, kRight>(right(next), t, vb);
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.full[c.step % kStages]);
+      return true;
     };
     settle();
-    float v[4][8];
-    if (next.live) fetch(next, v);
-    while (next.live) {
-      const Cursor c = next;
-      float now[4][8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) now[i][j] = v[i][j];
-      advance();
-      if (next.live) fetch(next, v);
-      const int st = c.step % kStages;
-      if (c.side == 0 && c.step >= kStages && !mbar_wait_warp(&S.empty[st], (c.step / kStages - 1) & 1, abort)) {
-        ok = false;
-        break;
-      }
-      put(c, now);
-      if (!WEIGHTS || c.side == 1) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.full[st]);
-      }
+    if (next.live) {
+      fetch<WEIGHTS ? 16 : 8, kLeft>(left(next), t, va);
+      if constexpr (WEIGHTS) fetch<kRightWide, kRight>(right(next), t, vb);
+    }
+    while (next.live && ok) {
+      ok = one(va, vb);
+      if (!WEIGHTS && ok && next.live) ok = one(vb, va);
     }
     if (!ok && lane == 0) *abort = 1;
   }
