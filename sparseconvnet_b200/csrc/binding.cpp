@@ -1271,8 +1271,11 @@ SCN_FN(adamw_step) {
   }
   int64_t *word = (int64_t *)written(step, at::kLong, step, 1, "step");
   std::vector<scn_adamw_tensor> table((size_t)params.n);
-  std::vector<at::Tensor> held, touched;
+  std::vector<at::Tensor> held;
+  std::vector<const at::Tensor *> touched;
   std::vector<void *> seen;
+  touched.reserve((size_t)params.n * 6 + 1);
+  seen.reserve((size_t)params.n * 6);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     scn_adamw_tensor &e = table[(size_t)i];
     const at::Tensor &p = params.at(i), &g = grads.at(i);
@@ -1280,25 +1283,25 @@ SCN_FN(adamw_step) {
     e.param = written(p, param_type, step, n, "params");
     if (g.scalar_type() != grad_type || g.sizes() != p.sizes() || g.device() != step.device())
       fail("grads must have the shapes of params, one type, and their device");
-    held.push_back(g.is_contiguous() ? g : g.contiguous());
-    e.grad = raw(held.back());
+    if (!g.is_contiguous()) held.push_back(g.contiguous());
+    e.grad = raw(g.is_contiguous() ? g : held.back());
     e.exp_avg = written(m.at(i), state_type, step, n, "exp_avgs");
     e.exp_avg_sq = written(v.at(i), state_type, step, n, "exp_avg_sqs");
-    touched.insert(touched.end(), {p, m.at(i), v.at(i)});
+    touched.insert(touched.end(), {&p, &m.at(i), &v.at(i)});
     e.exp_avg_scale = e.exp_avg_sq_scale = nullptr;
     if (ms.seq) {
       e.exp_avg_scale = (float *)written(ms.at(i), at::kFloat, step, blocks, "exp_avg_scales");
       e.exp_avg_sq_scale = (float *)written(vs.at(i), at::kFloat, step, blocks, "exp_avg_sq_scales");
-      touched.insert(touched.end(), {ms.at(i), vs.at(i)});
+      touched.insert(touched.end(), {&ms.at(i), &vs.at(i)});
     }
     e.copy = nullptr;
     if (copy_code >= 0) {
       e.copy = written(copies.at(i), copy_type, step, n, "copies");
-      touched.push_back(copies.at(i));
+      touched.push_back(&copies.at(i));
     }
   }
-  for (const at::Tensor &t : touched)
-    if (t.numel()) seen.push_back(t.data_ptr());
+  for (const at::Tensor *t : touched)
+    if (t->numel()) seen.push_back(t->data_ptr());
   std::sort(seen.begin(), seen.end());
   if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) fail("a tensor is in the lists twice");
   {
@@ -1306,9 +1309,9 @@ SCN_FN(adamw_step) {
     SCN_CALL(scn_adamw_step(table.data(), (int64_t)params.n, param_code, grad_code, bits, copy_code, word, lr, lr_dev, beta1, beta2,
                             eps, wd, (uint32_t)seed, on.stream));
   }
-  touched.push_back(step);
-  for (const at::Tensor &t : touched)  // whoever keeps something by a tensor's version sees that it was written
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  touched.push_back(&step);
+  for (const at::Tensor *t : touched)  // whoever keeps something by a tensor's version sees that it was written
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   Py_RETURN_NONE;
   SCN_END
 }

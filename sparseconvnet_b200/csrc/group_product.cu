@@ -194,6 +194,9 @@ __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap *map, 
       : "memory");
 }
 
+// a tensor map on its way into the cache that copies read it from
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 template <bool F8>
 __device__ __forceinline__ void mma_if(unsigned lead, unsigned d, unsigned a_lo, unsigned a_hi, unsigned b_lo, unsigned b_hi, unsigned idesc,
                                        unsigned accumulate) {
@@ -359,6 +362,7 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     S.issued = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 2 && lane == 0) prefetch_map(&map_a), prefetch_map(&map_b);
   if (warp == 1) tmem_alloc(&S.tmem, 512);
   scan_groups<WEIGHTS>(P, S);
   tc_fence_before();
@@ -626,6 +630,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     S.tails = S.tail_last = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 2 && lane == 0) prefetch_map(&map_a), prefetch_map(&map_b);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -976,6 +981,7 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
     S.issued = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (!WEIGHTS && warp == 2 && lane == 0) prefetch_map(&map_b);
   if (warp == 1) tmem_alloc(&S.tmem, 512);
   scan_groups<WEIGHTS>(P, S);
   tc_fence_before();
@@ -1206,33 +1212,46 @@ __device__ __forceinline__ void put_value(void *out, int type, long long at, flo
     ((__half *)out)[at] = __float2half_rn(v);
 }
 
-// The gradients of the groups of several units: their partial sums, in order
+// The gradients of the groups of several units: their partial sums.  32 results to a block, 8 threads to a result: each adds
+// every eighth unit, and their sums are added in order, so the result does not depend on timing (a group may have a hundred
+// times the units of the next: one thread to a result took 14 us where this takes 11).
 __global__ void __launch_bounds__(256)
 k_group_sum(const __grid_constant__ GroupParams P) {
   SCN_GRID_WAIT();
   __shared__ Shared S;
+  __shared__ float slices[8][32];
   scan_groups<true>(P, S);
-  const long long size = (long long)P.m_rows * P.n, weights = (long long)P.m * P.n;
-  for (int g = blockIdx.y; g < P.groups; g += gridDim.y) {
+  const long long size = (long long)P.m_rows * P.n, weights = (long long)P.m * P.n, pieces = (size + 31) / 32;
+  const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
+  for (long long item = blockIdx.x; item < pieces * P.groups; item += gridDim.x) {
+    const int g = (int)(item / pieces);
     if (S.part[g] < 0) continue;
+    const long long i = (item - g * pieces) * 32 + lane;
     const int units = S.first[g + 1] - S.first[g];
-    const float *from = P.partial + S.part[g] * size;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long long)gridDim.x * 256) {
-      float v = 0.f;
-      int u = 0;
-      for (; u + 8 <= units; u += 8) {  // (added in order, asked for at once)
-        float x[8];
+    const float *from = P.partial + S.part[g] * size + i;
+    float v = 0.f;
+    if (i < size) {
+      int u = slice;
+      for (; u + 24 < units; u += 32) {  // (added in order, asked for at once)
+        float x[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __ldg(from + (u + j) * size + i);
+        for (int j = 0; j < 4; ++j) x[j] = __ldg(from + (u + 8 * j) * size);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v += x[j];
+        for (int j = 0; j < 4; ++j) v += x[j];
       }
-      for (; u < units; ++u) v += __ldg(from + u * size + i);
+      for (; u < units; u += 8) v += __ldg(from + u * size);
+    }
+    slices[slice][lane] = v;
+    __syncthreads();
+    if (slice == 0 && i < size) {
+#pragma unroll
+      for (int j = 1; j < 8; ++j) v += slices[j][lane];
       if (i < weights)
         put_value(P.out, P.out_type, g * weights + i, v);
       else
         put_value(P.d_bias, P.out_type, (long long)g * P.n + i - weights, v);
     }
+    __syncthreads();
   }
 }
 
@@ -1478,9 +1497,8 @@ int chunk_of(long long n_rows, long long tiles) {
 }
 
 int sum_parts(GroupParams P, cudaStream_t stream) {
-  const long long size = (long long)P.m_rows * P.n;
-  const long long across = std::min<long long>(ceil_div(size, 256), 4 * kSms), groups = std::min<long long>(P.groups, ceil_div(8 * kSms, across));
-  SCN_LAUNCH(k_group_sum, dim3((unsigned)across, (unsigned)groups), 256, 0, stream, P);
+  const long long items = ceil_div((long long)P.m_rows * P.n, 32) * P.groups;
+  SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(items, 6 * kSms), 256, 0, stream, P);
   SCN_CUDA_CHECK(cudaGetLastError());
   return SCN_OK;
 }
