@@ -1212,46 +1212,61 @@ __device__ __forceinline__ void put_value(void *out, int type, long long at, flo
     ((__half *)out)[at] = __float2half_rn(v);
 }
 
-// The gradients of the groups of several units: their partial sums.  32 results to a block, 8 threads to a result: each adds
-// every eighth unit, and their sums are added in order, so the result does not depend on timing (a group may have a hundred
-// times the units of the next: one thread to a result took 14 us where this takes 11).
+// The gradients of the groups of several units: their partial sums, in an order that goes by the number of units alone.  Few
+// units: a thread adds a result's sums, 256 results to a block.  Many (a group may have a hundred times the units of the
+// next): 32 results to a block, 8 threads to a result, each adds every eighth unit, and their sums are added in order.  The
+// blocks are dealt to the pieces of all such groups in turn.
+constexpr int kManyUnits = 16;
 __global__ void __launch_bounds__(256)
 k_group_sum(const __grid_constant__ GroupParams P) {
   SCN_GRID_WAIT();
   __shared__ Shared S;
   __shared__ float slices[8][32];
   scan_groups<true>(P, S);
-  const long long size = (long long)P.m_rows * P.n, weights = (long long)P.m * P.n, pieces = (size + 31) / 32;
+  const long long size = (long long)P.m_rows * P.n, weights = (long long)P.m * P.n;
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
-  for (long long item = blockIdx.x; item < pieces * P.groups; item += gridDim.x) {
-    const int g = (int)(item / pieces);
+  auto store = [&](int g, long long i, float v) {
+    if (i < weights)
+      put_value(P.out, P.out_type, g * weights + i, v);
+    else
+      put_value(P.d_bias, P.out_type, (long long)g * P.n + i - weights, v);
+  };
+  long long turn = blockIdx.x;  // the first piece of the next such group that is this block's
+  for (int g = 0; g < P.groups; ++g) {
     if (S.part[g] < 0) continue;
-    const long long i = (item - g * pieces) * 32 + lane;
     const int units = S.first[g + 1] - S.first[g];
-    const float *from = P.partial + S.part[g] * size + i;
-    float v = 0.f;
-    if (i < size) {
-      int u = slice;
-      for (; u + 24 < units; u += 32) {  // (added in order, asked for at once)
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __ldg(from + (u + 8 * j) * size);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v += x[j];
+    const bool many = units >= kManyUnits;
+    const int each = many ? 32 : 256;
+    const long long pieces = (size + each - 1) >> (many ? 5 : 8);
+    const float *from = P.partial + S.part[g] * size;
+    for (; turn < pieces; turn += gridDim.x) {
+      const long long i = turn * each + (many ? lane : threadIdx.x);
+      const int step = many ? 8 : 1;
+      float v = 0.f;
+      if (i < size) {
+        const long long stride = step * size;
+        int u = many ? slice : 0;
+        const float *p = from + u * size + i;
+        for (; u + 3 * step < units; u += 4 * step, p += 4 * stride) {  // (added in order, asked for at once)
+          const float x0 = __ldg(p), x1 = __ldg(p + stride), x2 = __ldg(p + 2 * stride), x3 = __ldg(p + 3 * stride);
+          v += x0, v += x1, v += x2, v += x3;
+        }
+        for (; u < units; u += step, p += stride) v += __ldg(p);
       }
-      for (; u < units; u += 8) v += __ldg(from + u * size);
-    }
-    slices[slice][lane] = v;
-    __syncthreads();
-    if (slice == 0 && i < size) {
+      if (!many) {
+        if (i < size) store(g, i, v);
+        continue;
+      }
+      slices[slice][lane] = v;
+      __syncthreads();
+      if (slice == 0 && i < size) {
 #pragma unroll
-      for (int j = 1; j < 8; ++j) v += slices[j][lane];
-      if (i < weights)
-        put_value(P.out, P.out_type, g * weights + i, v);
-      else
-        put_value(P.d_bias, P.out_type, (long long)g * P.n + i - weights, v);
+        for (int j = 1; j < 8; ++j) v += slices[j][lane];
+        store(g, i, v);
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    turn -= pieces;
   }
 }
 
@@ -1498,7 +1513,7 @@ int chunk_of(long long n_rows, long long tiles) {
 
 int sum_parts(GroupParams P, cudaStream_t stream) {
   const long long items = ceil_div((long long)P.m_rows * P.n, 32) * P.groups;
-  SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(items, 6 * kSms), 256, 0, stream, P);
+  SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(items, 8 * kSms), 256, 0, stream, P);
   SCN_CUDA_CHECK(cudaGetLastError());
   return SCN_OK;
 }
