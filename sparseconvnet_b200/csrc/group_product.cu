@@ -124,7 +124,36 @@ __device__ __forceinline__ int over_before(int v, int *warp_sums) {
 // the rows behind and in front of all groups, whose results are zeros.
 template <bool WEIGHTS>
 __device__ __forceinline__ void scan_groups(const GroupParams &P, Shared &S) {
-  const int G = P.groups, tid = threadIdx.x, each = (G + 2 + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int G = P.groups, tid = threadIdx.x;
+  if (G + 2 <= 32) {  // one warp, without a barrier until the end: a call on 37 rows 8.4 -> 7.4 us
+    if (tid < 32) {
+      const int all = WEIGHTS ? G : G + 2;
+      int begin = tid <= G ? offset_at(P, tid) : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, begin, d);
+        if (tid >= d) begin = max(begin, o);
+      }
+      const int next = __shfl_down_sync(0xffffffffu, begin, 1), head = __shfl_sync(0xffffffffu, begin, 0);
+      const int end = tid < G ? next : tid == G ? P.n_rows : head;
+      if (tid > G) begin = 0;
+      const int units = tid < all ? units_of(P, WEIGHTS, end - begin) : 0, parts = units > 1 ? units : 0;
+      int upto = units, parts_upto = parts;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, d), q = __shfl_up_sync(0xffffffffu, parts_upto, d);
+        if (tid >= d) upto += o, parts_upto += q;
+      }
+      if (tid < all) {
+        S.begin[tid] = begin, S.end[tid] = end, S.first[tid] = upto - units;
+        if (tid == all - 1) S.first[all] = upto;
+        if (WEIGHTS) S.part[tid] = units > 1 ? parts_upto - parts : -1;
+      }
+    }
+    __syncthreads();
+    return;
+  }
+  const int each = (G + 2 + (int)blockDim.x - 1) / (int)blockDim.x;
   const int from = tid * each, to = min(from + each, G + 1);
   int most = 0;
   for (int g = from; g < to; ++g) most = max(most, S.begin[g] = offset_at(P, g));
@@ -167,7 +196,7 @@ struct Walk {
   __device__ __forceinline__ Unit at(long long u) {
     const int all = WEIGHTS ? P.groups : P.groups + 2;
     const int tiles = WEIGHTS ? P.n_tiles * P.m_tiles : P.n_tiles;
-    const int r = u >> 32 ? (int)(u / tiles) : (int)((unsigned)u / (unsigned)tiles), t = (int)(u - (long long)r * tiles);
+    const int r = tiles == 1 ? (int)u : u >> 32 ? (int)(u / tiles) : (int)((unsigned)u / (unsigned)tiles), t = (int)(u - (long long)r * tiles);
     for (int i = 0; i < 3 && S.first[group + 1] <= r; ++i) ++group;  // (first[all] is above every r)
     if (S.first[group + 1] <= r) {
       int lo = group + 1, hi = all - 1;  // the last group that begins at or before r: one without a unit shares its start with the next
@@ -181,7 +210,7 @@ struct Walk {
       group = lo;
     }
     const int each = WEIGHTS ? P.chunk : P.tile, row = S.begin[group] + (r - S.first[group]) * each;
-    const int m = WEIGHTS ? (int)((unsigned)t / (unsigned)P.n_tiles) : 0;
+    const int m = !WEIGHTS || t == 0 ? 0 : (int)((unsigned)t / (unsigned)P.n_tiles);
     return {group, row, min(each, S.end[group] - row), (t - m * P.n_tiles) * TN, m * P.tile,
             WEIGHTS && S.part[group] >= 0 ? S.part[group] + r - S.first[group] : -1};
   }

@@ -355,6 +355,27 @@ def test_a_wait_that_runs_out_is_reported(cuda):
         scn.poll_errors()
 
 
+def test_memory_that_runs_out(cuda):
+    """An allocation that fails ends the call with an error, and the next one is right."""
+    from sparseconvnet_b200._lib import lib
+    o = offsets_of([300, 500])
+    for t, k, n in ((torch.float32, 64, 96), (torch.float32, 300, 300), (torch.bfloat16, 63, 96)):
+        x, w, dy = normal(800, k, t=t, seed=1).requires_grad_(), normal(2, k, n, t=t, seed=2).requires_grad_(), normal(800, n, t=t, seed=3)
+        y = scn.grouped_product(x, w, o)
+        want = torch.autograd.grad(y, [x, w], dy, retain_graph=True)
+        for which in (1, 2, 3):
+            lib.scn_test_fail_allocation(which)
+            try:
+                with pytest.raises(Exception):
+                    scn.grouped_product(x.detach(), w.detach(), o)
+                    raise RuntimeError("fewer allocations than that")
+            finally:
+                lib.scn_test_fail_allocation(0)
+            assert torch.equal(scn.grouped_product(x, w, o), y)
+        got = torch.autograd.grad(y, [x, w], dy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_block_in_training(cuda):
     """Norm, grouped product and optimiser together, as a residual block over sites uses them: gradients against the same block in
     64 bits, and the optimiser's step on them."""
