@@ -21,6 +21,11 @@
 //               next tile is summed.
 //   roles       one warp copies tiles in (TMA, 128-byte swizzle, a ring over all of shared memory), one issues the
 //               instructions, eight read the accumulators, scale, add the bias, round and store.
+//   measured    32749 rows of 32 groups, 2048 -> 2048 bf16: forward and input gradient 202 us each (1360 TFLOP/s, the tensor
+//               cores busy 90% of the time at the 1.53 GHz that the power limit leaves), weights' gradient 262 (59%: a group's
+//               256 x 256 results cost as much to write as 500 rows to sum); 65536 rows, 4096 -> 2048 in 8 bits 378 us
+//               alone (2.9 PFLOP/s, 93%), 450 to 480 in a row; 37 rows of 8 groups, 1024 -> 1024: 8 us, two trips to L2
+//               behind 2 us of set-up; 131071 fp32 rows, 64 -> 96: 31, 35 and 50 us, bound by the splitting warps' latency.
 //   small groups  rows behind a group's last are not copied (boxes of 32 rows): their accumulator rows hold anything and are
 //               not stored.
 //
