@@ -6,10 +6,11 @@
 //     8 bits         y[r]  = s[r] S[g] (q[r] Q[g]) + b[g]        (e4m3 values, a scale per row and per group and output plane)
 //
 // The groups' sizes are known on the device only: every block sums the tiles of the groups before it looks for its own
-// (one scan at the start of the kernel), and takes every gridDim.x-th tile.  One kernel for all of them; what differs is
+// (one scan at the start of the kernel), and takes every gridDim.x-th tile.  k_group_product does all four; what differs is
 // which planes of an operand lie next to each other in memory (K-major: those that are summed over, M- / N-major: the
 // others) and, for the weights' gradient, that a tile's sum runs over rows and has to end inside a stage: there the rows
 // of the next group are overwritten with zeros before the tensor core sees them (0 times what stands there could be NaN).
+// k_group_pair takes wide layers and large groups, k_group_split fp32 rows of few planes.
 //
 //   arithmetic  16-bit and 8-bit values as they are, fp32 sums.  fp32 values as bf16 parts (k_group_parts): x = h + m + l
 //               holds all 24 bits, and the products h h, h m, m h, h l, l h, m m leave out 2^-24 of a product; two parts and
@@ -60,7 +61,6 @@ struct GroupParams {
   int n_tiles, m_tiles;    // m_tiles: weights only
   int chunk;               // weights: rows of a unit
   int tile;                // rows of a unit (rows) or of a tile of the result (weights)
-  int stages;
   unsigned idesc;          // without N
   void *out;
   int out_type, vectors, part_vectors;  // vectors_of the results and of the partial sums
@@ -102,7 +102,9 @@ __device__ __forceinline__ int offset_at(const GroupParams &P, int g) {
 }
 
 __device__ __forceinline__ int units_of(const GroupParams &P, bool weights, int rows) {
-  return weights ? max(1, (rows + P.chunk - 1) / P.chunk) : (rows + P.tile - 1) / P.tile;
+  const unsigned each = weights ? P.chunk : P.tile;  // (rows + each may pass 2^31)
+  const int units = (int)(((unsigned)rows + each - 1) / each);
+  return weights ? max(1, units) : units;
 }
 
 // Sum (or maximum) of v >= 0 over the threads before this one
