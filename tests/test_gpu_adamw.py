@@ -291,6 +291,22 @@ def test_writes_are_seen_by_version(cuda):
         y.backward()
 
 
+def test_more_than_2_31_values(cuda):
+    n = 2 ** 31 + 1000
+    st = {"params": [torch.zeros(n, device="cuda", dtype=torch.bfloat16)], "grads": [torch.zeros(n, device="cuda", dtype=torch.bfloat16)],
+          "exp_avgs": [torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)],
+          "exp_avg_sqs": [torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)],
+          "exp_avg_scales": [torch.zeros(-(-n // 256), device="cuda")], "exp_avg_sq_scales": [torch.zeros(-(-n // 256), device="cuda")]}
+    p, g = normal(1000, 1, torch.bfloat16), normal(1000, 2, torch.bfloat16)
+    st["params"][0][-1000:], st["grads"][0][-1000:] = p, g
+    zero = torch.zeros(1000, device="cuda")
+    scn.adamw_step(step=steps(0), **st, **HYPER)
+    want, _, _, _, update = formula(p, g, zero, zero, 1, **HYPER)
+    off = (st["params"][0][-1000:].double() - want).abs()
+    assert bool((off <= half(torch.bfloat16) * want.abs() * (1 + 1e-6) + 24 * E * update + 3 * E * want.abs()).all())
+    assert bool((st["params"][0][:1000] == 0).all()) and bool((st["exp_avgs"][0][-1000:].float() != 0).any())
+
+
 def test_refusals(cuda):
     def call(**k):
         st = make([64, 64], 32)

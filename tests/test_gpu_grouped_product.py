@@ -355,6 +355,26 @@ def test_a_wait_that_runs_out_is_reported(cuda):
         scn.poll_errors()
 
 
+def test_more_than_2_31_values(cuda):
+    for t, n, k, m in ((torch.bfloat16, 270001, 8192, 64), (torch.float32, 9000001, 256, 16), (torch.bfloat16, 9000001, 16, 256)):
+        o = offsets_of([n // 3, n - n // 3 - 4, 4])
+        x, w = torch.empty(n, k, device="cuda", dtype=t).normal_(), normal(3, k, m, t=t, seed=1)
+        x[-4:] = normal(4, k, t=t, seed=2)
+        y = scn.grouped_product(x, w, o)
+        near(y[-4:], x[-4:].double() @ w[2].double(), x[-4:].double().abs() @ w[2].double().abs(), room(k, t), t)
+        near(y[:4], x[:4].double() @ w[0].double(), x[:4].double().abs() @ w[0].double().abs(), room(k, t), t)
+        dy = torch.zeros(n, m, device="cuda", dtype=t)  # a gradient for the last rows only: exact sums of few terms
+        dy[-4:] = normal(4, m, t=t, seed=3)
+        x.requires_grad_()
+        w.requires_grad_()
+        dx, dw = torch.autograd.grad(scn.grouped_product(x, w, o), [x, w], dy)
+        d = dy[-4:].double()
+        near(dx[-4:], d @ w[2].detach().double().T, d.abs() @ w[2].detach().double().abs().T, room(m, t), t)
+        near(dw[2], x[-4:].detach().double().T @ d, x[-4:].detach().double().abs().T @ d.abs(), room(4, t), t)
+        assert bool((dw[:2] == 0).all()) and bool((dx[:8] == 0).all())
+        del x, y, dy, dx
+
+
 def test_memory_that_runs_out(cuda):
     """An allocation that fails ends the call with an error, and the next one is right."""
     from sparseconvnet_b200._lib import lib

@@ -236,6 +236,28 @@ def test_refusals(cuda):
     del y
 
 
+def test_more_than_2_31_values(cuda):
+    """Rows are independent, so those at the end have the bits that they have alone."""
+    n, c = 530001, 4096
+    x, r = torch.empty(n, c, device=cuda, dtype=torch.bfloat16).normal_(), rows(3, c, torch.bfloat16, 1)
+    x[-3:] = rows(3, c, torch.bfloat16, 2)
+    y, s = scn.rms_norm(x, residual=x)
+    want, sums = scn.rms_norm(x[-3:].clone(), residual=x[-3:].clone())
+    assert torch.equal(y[-3:], want) and torch.equal(s[-3:], sums)
+    del y, s
+    q, scale = scn.rms_norm_quantized(x)
+    want, scales = scn.rms_norm_quantized(x[-3:].clone())
+    assert torch.equal(q[-3:].float(), want.float()) and torch.equal(scale[-3:], scales)
+    del q
+    x.requires_grad_()
+    y = scn.rms_norm(x)
+    (gx,) = torch.autograd.grad(y, [x], y.detach())
+    part = x.detach()[-3:].clone().requires_grad_()
+    out = scn.rms_norm(part)
+    (want,) = torch.autograd.grad(out, [part], out.detach())
+    assert torch.equal(gx[-3:], want) and r.shape == want.shape
+
+
 def test_modules_over_sites(cuda):
     import numpy as np
     rng = np.random.default_rng(0)
