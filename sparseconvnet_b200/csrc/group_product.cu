@@ -688,7 +688,9 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   // ==== copies ====
   if (warp == 0) {
     const bool lead = elect_one();
-    int step = 0;
+    const unsigned full0 = in_block(&S.full[0], 0), ring0 = smem_u32(ring);
+    int step = 0, st = 0;
+    unsigned lap = 1;    // (a new barrier counts as past its phase of parity 1)
     unsigned tails = 0;  // a bit per stage, the other way round after each sum that ended there
     bool ok = true;
     Walk<WEIGHTS, kPairN> walk(P, S);
@@ -698,15 +700,14 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       constexpr unsigned kBox = WEIGHTS ? kStageRows * kRow : kTileM * kRow;
       const unsigned mine = boxes * kBox + kBBytes, both = (boxes_of(u, 0) + boxes_of(u, 1)) * kBox + 2 * kBBytes;
       for (int k = 0; k < steps; ++k, ++step) {
-        const int st = step % kStages;
-        if (step >= kStages && !wait_pair(&S.empty[st], (step / kStages - 1) & 1, abort)) {
+        if (!wait_pair(&S.empty[st], lap, abort)) {
           ok = false;
           break;
         }
         // a sum that ends inside a stage: each block sees its own copies land, to overwrite what lies behind the last row
         const bool tail = WEIGHTS && (k + 1) * kStageRows > u.rows;
         if (lead) {
-          const unsigned a = smem_u32(ring) + st * kStage, b = a + kABytes, bar = tail ? in_block(&S.tail[st], rank) : in_block(&S.full[st], 0);
+          const unsigned a = ring0 + st * kStage, b = a + kABytes, bar = tail ? in_block(&S.tail[st], rank) : full0 + st * 8;
           if (tail) {
             mbar_expect_tx(&S.tail[st], mine);
             if (rank == 0) mbar_arrive(&S.full[st]);
@@ -727,6 +728,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           S.issued = step + 1;
         }
         if (tail) tails ^= 1u << st;
+        if (++st == kStages) st = 0, lap ^= 1;
         __syncwarp();
       }
     }
@@ -734,9 +736,9 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   }
   // ==== instructions ====
   else if (warp == 1) {
-    const unsigned lead = elect_one();
-    int step = 0, turn = 0;
-    unsigned tails = 0;
+    const unsigned lead = elect_one(), ring0 = smem_u32(ring);
+    int step = 0, turn = 0, st = 0;
+    unsigned lap = 0, tails = 0;
     bool ok = true;
     Walk<WEIGHTS, kPairN> walk(P, S);
     for (long long i = pair; i < units && ok; i += pairs) {
@@ -748,8 +750,8 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         ok = false;
         break;
       }
-      for (int k = 0; k < steps; ++k, ++step) {
-        const int st = step % kStages;
+      const unsigned d = tmem + (turn & 1) * kColumns;
+      for (int k = 0; k < steps; ++k, ++step, lap ^= st == kStages - 1, st = st == kStages - 1 ? 0 : st + 1) {
         int instructions = 4;
         if (WEIGHTS && behind && k == steps - 1) {
           instructions = (behind + 15) / 16;
@@ -770,13 +772,15 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           tails ^= 1u << st;
         }
         if (rank != 0) continue;
-        if (!wait_pair(&S.full[st], (step / kStages) & 1, abort)) {
+        if (!wait_pair(&S.full[st], lap, abort)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const unsigned a = smem_u32(ring) + st * kStage, b = a + kABytes, d = tmem + (turn & 1) * kColumns;
-        for (int j = 0; j < instructions; ++j) {
+        const unsigned a = ring0 + st * kStage, b = a + kABytes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= instructions) break;
           const unsigned pa = a + j * (WEIGHTS ? 16 * kRow : 32), pb = b + j * (WEIGHTS || B_ROWS ? 16 * kRow : 32);
           mma_pair_if<F8>(lead, d, desc_lo(pa, WEIGHTS ? kStageRows * kRow : 16), kDescHi, desc_lo(pb, WEIGHTS || B_ROWS ? kStageRows * kRow : 16), kDescHi,
                           idesc, k > 0 || j > 0);
