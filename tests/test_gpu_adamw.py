@@ -265,6 +265,34 @@ def test_optimizer_against_torch(cuda, bits):
         assert float((p - q).detach().abs().max()) < (6 * 2e-2 * 2 * (100 * E if bits == 32 else 0.5))
 
 
+def test_no_tensors(cuda):
+    """A list of nothing, or of tensors without values, is a step all the same."""
+    step = steps(4)
+    scn.adamw_step([], [], [], [], step)
+    empty = [torch.zeros(0, device="cuda")] * 2
+    scn.adamw_step(empty, empty, empty, empty, step)
+    assert int(step) == 6
+
+
+def test_a_checkpoint_in_a_file(cuda, tmp_path):
+    """States go through a file with their types, and the run goes on as it would have."""
+    runs = []
+    for through_file in (False, True):
+        p = torch.nn.Parameter(normal(3000, 1, torch.bfloat16))
+        opt = scn.AdamW([p], lr=1e-2, state_bits=8, master_weights=True, seed=3)
+        for k in range(4):
+            p.grad = normal(3000, 10 + k, torch.bfloat16)
+            opt.step()
+            if through_file and k == 1:
+                torch.save(opt.state_dict(), tmp_path / "state")
+                opt = scn.AdamW([p], lr=1e-2, state_bits=8, master_weights=True, seed=3)
+                opt.load_state_dict(torch.load(tmp_path / "state"))
+        runs.append((p.detach(), opt.state[p]))
+    assert torch.equal(runs[0][0], runs[1][0])
+    for k, v in runs[0][1].items():
+        assert v.dtype == runs[1][1][k].dtype and torch.equal(v.float(), runs[1][1][k].float()), k
+
+
 def test_master_weights(cuda):
     """Updates below half a step of bfloat16 add up in the fp32 weights."""
     p = torch.nn.Parameter(torch.ones(512, device="cuda", dtype=torch.bfloat16))
