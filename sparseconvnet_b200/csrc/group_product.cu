@@ -63,10 +63,9 @@ struct GroupParams {
   int tile;                // rows of a unit (rows) or of a tile of the result (weights)
   unsigned idesc;          // without N
   void *out;
-  int out_type, vectors, part_vectors;  // vectors_of the results and of the partial sums
+  int out_type, aligned, part_aligned;  // what the results' and the partial sums' rows are aligned to
   int m_rows;              // weights: rows of the result with that of the bias sums, if a tile has room for it
   void *d_bias;
-  int bias_vectors;
   const float *a, *b;      // fp32 operands that the kernel splits itself
   long long a_stride, b_stride;
   int a_quads, b_quads;    // their rows take 16-byte loads
@@ -84,7 +83,7 @@ struct Shared {
   int abort, issued;
   unsigned tails, tail_last;  // stages that have been a sum's end, and the parity of the last time
   int warp_sums[32];
-  __align__(16) float columns[kEpilogueWarps][32];
+  __align__(16) float columns[kEpilogueWarps][128];
   int first[kMostGroups + 3];  // units (of rows) before the group
   int begin[kMostGroups + 2], end[kMostGroups + 2];
   int part[kMostGroups];       // weights: units before the group among the groups of several units, -1: one unit
@@ -265,57 +264,81 @@ __device__ __forceinline__ float value_at(const void *p, int type, long long i) 
                                      : __half2float(__ldg((const __half *)p + i));
 }
 
-// 32 results of a row from column c on.  vectors 2: whole sectors of 32 bytes (pieces of 16 bytes reach L2 as two writes of half
-// a sector: group_wide_8bit took 40 us more), 1: pieces of 16 bytes, 0: one by one.
-__device__ __forceinline__ void store8w(void *p, int vectors, const unsigned *w) {
-  if (vectors == 2) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
-                 "r"(w[6]), "r"(w[7])
-                 : "memory");
+// 32 results of a row, `left` of them in the row, in rows that begin at multiples of `aligned` bytes: 8, 16 or 32.  32: whole
+// sectors (pieces of 16 bytes reach L2 as two writes of half a sector: group_wide_8bit took 70 us more).
+template <int WORDS>
+__device__ __forceinline__ void store_words32(void *to, int aligned, int left, const unsigned (&w)[WORDS]) {
+  constexpr int kPer = 32 / WORDS;  // values of a word
+  unsigned *q = (unsigned *)to;
+  if (left >= 32 && aligned == 32) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]),
+                   "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                   : "memory");
+  } else if (aligned >= 16) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4)
+      if (i * kPer < left) *reinterpret_cast<uint4 *>(q + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   } else {
-    reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 2)
+      if (i * kPer < left) *reinterpret_cast<uint2 *>(q + i) = make_uint2(w[i], w[i + 1]);
   }
 }
-__device__ __forceinline__ void store32(void *out, int type, int vectors, long long at, int left, const float (&v)[32]) {
-  if (vectors && left >= 32) {
-    if (type == SCN_TYPE_FLOAT32) {
+// The same for rows that begin anywhere: through 512 bytes of shared memory, so that a warp writes a row's values side by side (a
+// lane that writes its row value by value touches 32 lines with every store: 60000 x 257 -> 333 bf16 took 316 us, now 82).  `to`: the
+// lane's row, null if it is not stored.
+template <int WORDS>
+__device__ __forceinline__ void store_words32_anywhere(void *to, int left, const unsigned (&w)[WORDS], unsigned *shared) {
+  constexpr int kRows = 128 / WORDS;  // rows at a time
+  const int lane = threadIdx.x % 32;
+#pragma unroll 1
+  for (int q = 0; q < 32; q += kRows) {
+    if (lane >= q && lane < q + kRows) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        unsigned w[8];
+      for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4 *>(shared + (lane - q) * WORDS + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
-        store8w((float *)out + at + 8 * i, vectors, w);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        unsigned w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          w[j] = type == SCN_TYPE_BFLOAT16 ? pair(v[16 * i + 2 * j], v[16 * i + 2 * j + 1], __nv_bfloat16())
-                                           : pair(v[16 * i + 2 * j], v[16 * i + 2 * j + 1], __half());
-        store8w((unsigned short *)out + at + 16 * i, vectors, w);
+    for (int r = 0; r < kRows; ++r) {
+      void *row = (void *)__shfl_sync(0xffffffffu, (unsigned long long)to, q + r);
+      if (row && lane < left) {
+        if (WORDS == 32)
+          ((unsigned *)row)[lane] = shared[r * WORDS + lane];
+        else
+          ((unsigned short *)row)[lane] = ((const unsigned short *)shared)[r * 32 + lane];
       }
     }
-    return;
+    __syncwarp();
   }
+}
+// The whole warp comes here.
+__device__ __forceinline__ void store32(void *to, int type, int aligned, int left, const float (&v)[32], float *shared) {
+  if (type == SCN_TYPE_FLOAT32) {
+    unsigned w[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (i >= left) break;
-    if (type == SCN_TYPE_FLOAT32)
-      ((float *)out)[at + i] = v[i];
-    else if (type == SCN_TYPE_BFLOAT16)
-      ((__nv_bfloat16 *)out)[at + i] = __float2bfloat16_rn(v[i]);
-    else
-      ((__half *)out)[at + i] = __float2half_rn(v[i]);
+    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+    if (aligned < 8)
+      store_words32_anywhere(to, left, w, (unsigned *)shared);
+    else if (to)
+      store_words32(to, aligned, left, w);
+  } else {
+    unsigned w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = type == SCN_TYPE_BFLOAT16 ? pair(v[2 * i], v[2 * i + 1], __nv_bfloat16()) : pair(v[2 * i], v[2 * i + 1], __half());
+    if (aligned < 8)
+      store_words32_anywhere(to, left, w, (unsigned *)shared);
+    else if (to)
+      store_words32(to, aligned, left, w);
   }
 }
 
-// Values of `bytes` in rows of n: how store32 may write them (a row begins at a multiple of n, a run of 32 at a multiple of 32)
-__host__ __device__ inline int vectors_of(uintptr_t p, long long n, int bytes) {
+// Values of `bytes` in rows of n from p on: what every row's results are aligned to (a run of 32 begins at a multiple of 32)
+__host__ __device__ inline int aligned_to(uintptr_t p, long long n, int bytes) {
   const uintptr_t all = p | (uintptr_t)(n * bytes);
-  return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
+  return all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : bytes;
 }
 
 // What belongs to a unit's columns and rows, read by a warp of the epilogue while the unit is still being summed: lane l has
@@ -338,7 +361,7 @@ struct Terms {
   }
 };
 
-// 32 results of the row `lane_row` of a unit, from column c = c0 + 32 j on; the whole warp comes here.  `shared`: 32 floats of the
+// 32 results of the row `lane_row` of a unit, from column c = c0 + 32 j on; the whole warp comes here.  `shared`: 128 floats of the
 // warp, through which every lane sees all columns' terms.
 template <int COLS, bool WEIGHTS, bool F8>
 __device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, const Terms<COLS, WEIGHTS, F8> &terms, int j, int lane_row, int c,
@@ -364,18 +387,17 @@ __device__ __forceinline__ void finish32(const GroupParams &P, const Unit &u, co
     }
     __syncwarp();
   }
+  auto at = [&](void *p, int type, long long row) { return (void *)((char *)p + (row * P.n + c) * (type == SCN_TYPE_FLOAT32 ? 4 : 2)); };
   if (WEIGHTS) {
     const int m = u.m0 + lane_row;
-    if (m >= P.m_rows) return;
-    if (u.part >= 0)
-      store32(P.partial, SCN_TYPE_FLOAT32, P.part_vectors, ((long long)u.part * P.m_rows + m) * P.n + c, P.n - c, v);
-    else if (m < P.m)
-      store32(P.out, P.out_type, P.vectors, ((long long)u.group * P.m + m) * P.n + c, P.n - c, v);
-    else
-      store32(P.d_bias, P.out_type, P.bias_vectors, (long long)u.group * P.n + c, P.n - c, v);
-    return;
+    const bool part = u.part >= 0;
+    const int type = part ? (int)SCN_TYPE_FLOAT32 : P.out_type;
+    void *to = nullptr;
+    if (m < P.m_rows) to = part ? at(P.partial, type, (long long)u.part * P.m_rows + m) : m < P.m ? at(P.out, type, (long long)u.group * P.m + m) : at(P.d_bias, type, u.group);
+    store32(to, type, part ? P.part_aligned : P.aligned, P.n - c, v, shared);
+  } else {
+    store32(lane_row < u.rows ? at(P.out, P.out_type, u.row + lane_row) : nullptr, P.out_type, P.aligned, P.n - c, v, shared);
   }
-  if (lane_row < u.rows) store32(P.out, P.out_type, P.vectors, (long long)(u.row + lane_row) * P.n + c, P.n - c, v);
 }
 
 template <int PARTS, int TN, bool SUMS, bool WEIGHTS, bool B_ROWS, bool F8>
@@ -1324,11 +1346,11 @@ k_group_bias(const __grid_constant__ GroupParams P, const void *d_out, long long
     float v = 0.f;
     if (c < P.n) {
       int r = along;
-      for (; r + 24 < unit.rows; r += 32) {
-        float x[4];
+      for (; r + 56 < unit.rows; r += 64) {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = value_at(d_out, type, (long long)(unit.row + r + 8 * j) * stride + c);
-        v += (x[0] + x[1]) + (x[2] + x[3]);
+        for (int j = 0; j < 8; ++j) x[j] = value_at(d_out, type, (long long)(unit.row + r + 8 * j) * stride + c);
+        v += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
       }
       for (; r < unit.rows; r += 8) v += value_at(d_out, type, (long long)(unit.row + r) * stride + c);
     }
@@ -1522,7 +1544,7 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(type, false, b_rows, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
-  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_size), P.part_vectors = vectors_of(0, n, 4);
+  P.out = out, P.out_type = out_type, P.aligned = aligned_to((uintptr_t)out, n, out_size), P.part_aligned = aligned_to(0, n, 4);
   P.bias = bias, P.bias_type = bias_type, P.row_scale = row_scale, P.col_scale = col_scale, P.drop = drop;
   const int per = f8 ? 128 : 64;
   CUtensorMap a, b;
@@ -1573,7 +1595,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
   P.idesc = idesc_of(type, true, true, P.tile);
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
-  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_size), P.part_vectors = vectors_of(0, n, 4);
+  P.out = out, P.out_type = out_type, P.aligned = aligned_to((uintptr_t)out, n, out_size), P.part_aligned = aligned_to(0, n, 4);
   const bool split = G.n_rows > P.chunk;
   // (a group of several units has more than P.chunk rows: at most n_rows / chunk of them, with one unit more each than that)
   if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * m * n));
@@ -1622,7 +1644,7 @@ int rows_product_split(const Groups &G, const void *x, long long stride, const O
   P.tile = kTileM;
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(SCN_TYPE_BFLOAT16, false, b_rows, kTileM);
-  P.out = out, P.out_type = out_type, P.vectors = vectors_of((uintptr_t)out, n, out_type == SCN_TYPE_FLOAT32 ? 4 : 2);
+  P.out = out, P.out_type = out_type, P.aligned = aligned_to((uintptr_t)out, n, out_type == SCN_TYPE_FLOAT32 ? 4 : 2);
   P.bias = bias, P.bias_type = bias_type, P.drop = drop;
   P.a = (const float *)x, P.a_stride = stride, P.a_quads = quads_of(x, stride, k);
   CUtensorMap b;
@@ -1648,8 +1670,9 @@ int weights_product_split(const Groups &G, const void *x, long long x_stride, co
   P.m = m, P.m_rows = m + *bias_done, P.n = n, P.m_tiles = (int)ceil_div(m, kTileM), P.n_tiles = (int)ceil_div(n, tn);
   P.chunk = kSplitSteps * kStageRows;
   P.idesc = idesc_of(SCN_TYPE_BFLOAT16, true, true, kTileM);
-  P.out = out, P.out_type = SCN_TYPE_FLOAT32, P.vectors = vectors_of((uintptr_t)out, n, 4), P.part_vectors = vectors_of(0, n, 4);
-  P.d_bias = *bias_done ? d_bias : nullptr, P.bias_vectors = vectors_of((uintptr_t)d_bias, n, 4);
+  P.out = out, P.out_type = SCN_TYPE_FLOAT32, P.aligned = aligned_to((uintptr_t)out, n, 4), P.part_aligned = aligned_to(0, n, 4);
+  P.d_bias = *bias_done ? d_bias : nullptr;
+  if (*bias_done) P.aligned = std::min(P.aligned, aligned_to((uintptr_t)d_bias, n, 4));
   P.a = (const float *)x, P.a_stride = x_stride, P.a_quads = quads_of(x, x_stride, m);
   P.b = (const float *)dy, P.b_stride = dy_stride, P.b_quads = quads_of(dy, dy_stride, n);
   const bool split = G.n_rows > P.chunk;
