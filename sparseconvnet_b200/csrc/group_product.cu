@@ -1332,9 +1332,14 @@ k_group_sum(const __grid_constant__ GroupParams P) {
   }
 }
 
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+
 // db[g] = sum of a group's rows: a block takes a unit of P.chunk rows and 32 planes, 8 rows at a time (m = 1)
+template <typename T>
 __global__ void __launch_bounds__(256)
-k_group_bias(const __grid_constant__ GroupParams P, const void *d_out, long long stride, int type) {
+k_group_bias(const __grid_constant__ GroupParams P, const T *__restrict__ d_out, long long stride) {
   SCN_GRID_WAIT();
   __shared__ Shared S;
   __shared__ float part[8][33];
@@ -1349,10 +1354,10 @@ k_group_bias(const __grid_constant__ GroupParams P, const void *d_out, long long
       for (; r + 56 < unit.rows; r += 64) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = value_at(d_out, type, (long long)(unit.row + r + 8 * j) * stride + c);
+        for (int j = 0; j < 8; ++j) x[j] = as_float(__ldg(d_out + (unit.row + r + 8 * j) * stride + c));
         v += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
       }
-      for (; r < unit.rows; r += 8) v += value_at(d_out, type, (long long)(unit.row + r) * stride + c);
+      for (; r < unit.rows; r += 8) v += as_float(__ldg(d_out + (unit.row + r) * stride + c));
     }
     part[along][lane] = v;
     __syncthreads();
@@ -1692,7 +1697,13 @@ int bias_sums(const Groups &G, const void *dy, long long stride, int type, int n
   const bool split = G.n_rows > P.chunk;
   if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * n));
   const long long units = ceil_div(G.n_rows, P.chunk) + G.groups;
-  SCN_LAUNCH(k_group_bias, dim3((unsigned)ceil_div(n, 32), (unsigned)std::min<long long>(units, 1024)), 256, 0, stream, P, dy, stride, type);
+  const dim3 grid((unsigned)ceil_div(n, 32), (unsigned)std::min<long long>(units, 1024));
+  if (type == SCN_TYPE_FLOAT32)
+    SCN_LAUNCH(k_group_bias<float>, grid, 256, 0, stream, P, (const float *)dy, stride);
+  else if (type == SCN_TYPE_BFLOAT16)
+    SCN_LAUNCH(k_group_bias<__nv_bfloat16>, grid, 256, 0, stream, P, (const __nv_bfloat16 *)dy, stride);
+  else
+    SCN_LAUNCH(k_group_bias<__half>, grid, 256, 0, stream, P, (const __half *)dy, stride);
   SCN_CUDA_CHECK(cudaGetLastError());
   return split ? sum_parts(P, stream) : SCN_OK;
 }
