@@ -420,8 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_dweight_tile(const __grid_const
           unsigned a[16], b[16], c[16];
           tmem_ld16_nowait(d + c0, a);
           tmem_ld16_nowait(d + PG + c0, b);
-          if (PG == 32) tmem_ld16_nowait(d + 2 * PG + c0, c);
-          tmem_wait_ld();
+          if (PG == 32) {
+            tmem_ld16_nowait(d + 2 * PG + c0, c);
+            tmem_wait_ld(a, b, c);
+          } else {
+            tmem_wait_ld(a, b);
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x = __uint_as_float(b[e]);

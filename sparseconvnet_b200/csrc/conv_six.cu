@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(SixWarps<NA>::THREADS, 1) k_conv_six(const __g
             if (!kJoint) {
               unsigned a[16];
               tmem_ld16_nowait(base + u * 16, a);
-              tmem_wait_ld();
+              tmem_wait_ld(a);
 #pragma unroll
               for (int e = 0; e < 16; ++e) acc[u * 16 + e] += __uint_as_float(a[e]);
             } else {
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(SixWarps<NA>::THREADS, 1) k_conv_six(const __g
                 tmem_ld8_nowait(base + u * 16 + e0, a);
                 tmem_ld8_nowait(base + cb + u * 16 + e0, b);
                 tmem_ld8_nowait(base + 2 * cb + u * 16 + e0, c);
-                tmem_wait_ld();
+                tmem_wait_ld(a, b, c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   acc[u * 16 + e0 + e] += __uint_as_float(a[e]) + (__uint_as_float(b[e]) + __uint_as_float(c[e]));

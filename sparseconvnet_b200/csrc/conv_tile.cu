@@ -134,7 +134,10 @@ __device__ __forceinline__ void store_columns(const TileParams &P, bool joint, u
       unsigned a[8], b[8];
       tmem_ld8_nowait(base + c0 + half, a);
       if (joint) tmem_ld8_nowait(base + P.coutp + c0 + half, b);
-      tmem_wait_ld();
+      if (joint)
+        tmem_wait_ld(a, b);
+      else
+        tmem_wait_ld(a);
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
         float4 v;

@@ -123,17 +123,17 @@ __device__ __forceinline__ void tc_mma(unsigned d_tmem, unsigned long long a_des
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 lanes x 16 consecutive 32-bit columns: thread t of the warp gets lane (base lane + t).
+// 32 lanes x 16 consecutive 32-bit columns: thread t of the warp gets lane (base lane + t).  The wait belongs to the load's own
+// statement: the compiler may move what reads the registers above a wait in a statement that does not name them.
 __device__ __forceinline__ void tmem_ld16(unsigned taddr, float *v) {
   unsigned r[16];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
+      "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -142,14 +142,13 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v) {
   unsigned r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -248,7 +247,18 @@ __device__ __forceinline__ void tmem_ld8_nowait(unsigned taddr, unsigned (&r)[8]
                : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Every load's registers are named here, so that what reads them stays behind the wait.
+template <int N>
+__device__ __forceinline__ void tmem_arrived(unsigned (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <int... N>
+__device__ __forceinline__ void tmem_wait_ld(unsigned (&...r)[N]) {
+  static_assert(sizeof...(N) > 0, "registers");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  (tmem_arrived(r), ...);
+}
 
 // Two floats as a bf16 pair rounded to nearest (`a` in the low half) and the pair of what the
 // rounding left over, again as bf16: the two parts of the three-term bf16 split.
