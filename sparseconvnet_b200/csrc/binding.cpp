@@ -1448,6 +1448,7 @@ SCN_FN(grouped_product_quantized) {
   }
   for (const at::Tensor *t : {&scale, &weight, &weight_scale, (const at::Tensor *)&bias})
     if (t->defined() && t->device() != q.device()) fail("all operands must be on the rows' device");
+  no_tangents(q, scale, weight, weight_scale, bias);
   if (ag::compute_requires_grad(scale, weight_scale, bias)) fail("a product of 8-bit rows has no gradient: call it under torch.no_grad()");
   const at::NoGradGuard no_grad;
   const at::Tensor rows = as_rows(q), s = scale.contiguous(), w = weight.contiguous(), ws = weight_scale.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
