@@ -44,6 +44,17 @@ def _state_of(p, bits):
     return made
 
 
+def _check_group(group):
+    if not isinstance(group["lr"], torch.Tensor) and not group["lr"] >= 0:
+        raise ValueError("lr must not be negative")
+    if not (0 <= group["betas"][0] < 1 and 0 <= group["betas"][1] < 1):
+        raise ValueError("betas must lie in [0, 1)")
+    if not group["eps"] >= 0 or not group["weight_decay"] >= 0:
+        raise ValueError("eps and weight_decay must not be negative")
+    if group["state_bits"] not in (8, 32):
+        raise ValueError("state_bits must be 8 or 32")
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update on the GPU in one launch for all parameters of a group.
 
@@ -54,16 +65,15 @@ class AdamW(torch.optim.Optimizer):
     step is not counted.  There is no amsgrad, no maximize and no CPU path."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
-        if not isinstance(lr, torch.Tensor) and not lr >= 0:
-            raise ValueError("lr must not be negative")
-        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
-            raise ValueError("betas must lie in [0, 1)")
-        if not eps >= 0 or not weight_decay >= 0:
-            raise ValueError("eps and weight_decay must not be negative")
-        if state_bits not in (8, 32):
-            raise ValueError("state_bits must be 8 or 32")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      master_weights=master_weights, seed=seed))
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights, seed=seed)
+        _check_group(defaults)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group):
+        """As torch's; a group's own values are checked like the constructor's."""
+        if isinstance(param_group, dict):
+            _check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _start(self, p, group):
         state = _state_of(p, group["state_bits"])
