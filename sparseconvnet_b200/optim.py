@@ -124,9 +124,34 @@ class AdamW(torch.optim.Optimizer):
                 for p in ps:
                     self.state[p]["step"] = own
 
+    def _check_checkpoint(self, state_dict):
+        saved = state_dict["param_groups"]
+        if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
+            return  # (torch refuses it)
+        for s, group in zip(saved, self.param_groups):
+            missing = sorted(set(self.defaults) - set(s))
+            if missing:
+                raise ValueError("the checkpoint is another optimizer's: a group of it has no %s" % ", ".join(missing))
+            _check_group(s)
+            for i, p in zip(s["params"], group["params"]):
+                state = state_dict["state"].get(i)
+                if not state:
+                    continue
+                n, master = p.numel(), s["master_weights"] and p.dtype != torch.float32
+                moments = (torch.float32, n) if s["state_bits"] == 32 else (torch.float8_e4m3fn, n)
+                want = dict(exp_avg=moments, exp_avg_sq=moments, step=(torch.int64, 1))
+                if s["state_bits"] == 8:
+                    want.update(exp_avg_scale=(torch.float32, -(-n // BLOCK)), exp_avg_sq_scale=(torch.float32, -(-n // BLOCK)))
+                if master:
+                    want["master"] = (torch.float32, n)
+                have = {k: (v.dtype, v.numel()) if isinstance(v, torch.Tensor) else v for k, v in state.items()}
+                if have != want:
+                    raise ValueError("the checkpoint does not fit parameter %s: it holds %s, %s expected" % (i, have, want))
+
     def load_state_dict(self, state_dict):
         """As torch's, but states keep their types (torch casts them to the parameter's), and parameters with the same count
-        share a counter again."""
+        share a counter again.  A checkpoint of another optimizer, or of parameters of other sizes, is refused."""
+        self._check_checkpoint(state_dict)
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             counters = {}
