@@ -55,6 +55,11 @@ def _check_group(group):
         raise ValueError("state_bits must be 8 or 32")
 
 
+def _not_captured(p, what):
+    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("AdamW cannot capture %s.  Take such a step before the capture." % what)
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update on the GPU in one launch for all parameters of a group.
 
@@ -62,7 +67,7 @@ class AdamW(torch.optim.Optimizer):
     master_weights: for bfloat16 / float16 parameters, keep them in float32 as well and round the parameters from those;
     without it an update smaller than half a step of the parameter's type is lost.
     lr of a group may be a float32 CUDA tensor of one value.  Parameters without a gradient are left as they are, and their
-    step is not counted.  There is no amsgrad, no maximize and no CPU path."""
+    step is not counted.  A step can be captured into a graph after the same parameters have taken one outside.  There is no amsgrad, no maximize and no CPU path."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False, seed=0):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights, seed=seed)
@@ -97,6 +102,7 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW does not take sparse gradients")
                 state = self.state[p]
                 if not state:
+                    _not_captured(p, "a parameter's first step: its moments would begin anew with every replay")
                     state.update(self._start(p, group))
                     if p.device not in fresh:
                         fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
@@ -120,6 +126,7 @@ class AdamW(torch.optim.Optimizer):
                 users.setdefault(id(self.state[p]["step"]), []).append(p)
         for key, ps in together.items():
             if len(users[key[0]]) > len(ps):
+                _not_captured(ps[0], "a step of some of the parameters that have stepped together: their count would begin anew with every replay")
                 own = self.state[ps[0]]["step"].clone()
                 for p in ps:
                     self.state[p]["step"] = own
