@@ -55,13 +55,17 @@ def _check_group(group):
         raise ValueError("state_bits must be 8 or 32")
 
 
+def _captures(p):
+    return p.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def _not_captured(p, what):
-    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+    if _captures(p):
         raise RuntimeError("AdamW cannot capture %s.  Take such a step before the capture." % what)
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's update on the GPU in one launch for all parameters of a group.
+    """torch.optim.AdamW's update on the GPU, one launch for all parameters of a group that have one type and as many steps.
 
     state_bits: 32, or 8 for moments of 8 bits with a scale per 256 values (2.03 bytes a value instead of 8).
     master_weights: for bfloat16 / float16 parameters, keep them in float32 as well and round the parameters from those;
@@ -93,43 +97,79 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for number, group in enumerate(self.param_groups):
-            fresh = {}    # device -> the counter of parameters that take their first step now
-            together = {}  # parameters that step as one list: one counter, one device, one type
+            fresh = {}     # device -> the counter of parameters that take their first step now
+            keys = {}      # counter -> its count where the host knows it, and its device
+            users = {}     # counter -> how many parameters have it
+            together = {}  # parameters that step as one list: one count, one device, one type -> they and their states
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
+                    state = self.state.get(p)
+                    if state:
+                        users[id(state["step"])] = users.get(id(state["step"]), 0) + 1
                     continue
-                if p.grad.is_sparse:
+                if grad.is_sparse:
                     raise RuntimeError("AdamW does not take sparse gradients")
                 state = self.state[p]
                 if not state:
                     _not_captured(p, "a parameter's first step: its moments would begin anew with every replay")
                     state.update(self._start(p, group))
                     if p.device not in fresh:
-                        fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
+                        fresh[p.device] = self._note(torch.zeros(1, dtype=torch.int64, device=p.device), 0)
                     state["step"] = fresh[p.device]
-                together.setdefault((id(state["step"]), p.dtype, p.grad.dtype, "master" in state), []).append(p)
-            self._one_counter_per_list(group, together)
-            for (_, _, _, master), ps in together.items():
-                states = [self.state[p] for p in ps]
+                step = id(state["step"])
+                users[step] = users.get(step, 0) + 1
+                if step not in keys:
+                    keys[step] = (self._count(state["step"]), p.device)
+                    if keys[step][0] is None:
+                        keys[step] = (None, step)
+                ps, states = together.setdefault((keys[step], p.dtype, grad.dtype, "master" in state), ([], []))
+                ps.append(p)
+                states.append(state)
+            for ((count, _), _, _, master), (ps, states) in together.items():
+                step = self._one_counter(ps, states, users)
                 column = lambda k: [s[k] for s in states] if k in states[0] else None  # noqa: E731
                 adamw_step(column("master") if master else ps, [p.grad for p in ps], column("exp_avg"), column("exp_avg_sq"),
-                           states[0]["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                           step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                            column("exp_avg_scale"), column("exp_avg_sq_scale"), group["seed"] + number, ps if master else None)
+                self._note(step, None if count is None or _captures(ps[0]) else count + 1)
         return loss
 
-    def _one_counter_per_list(self, group, together):
-        """A counter is advanced by the one list that has it: parameters that share it but step in another list, or not at all
-        this time, keep the old count in a counter of their own."""
-        users = {}
-        for p in group["params"]:
-            if self.state.get(p):
-                users.setdefault(id(self.state[p]["step"]), []).append(p)
-        for key, ps in together.items():
-            if len(users[key[0]]) > len(ps):
-                _not_captured(ps[0], "a step of some of the parameters that have stepped together: their count would begin anew with every replay")
-                own = self.state[ps[0]]["step"].clone()
-                for p in ps:
-                    self.state[p]["step"] = own
+    # What the host knows of the counters on the device, so that parameters whose counts have become equal step as one list
+    # again: id -> (counter, its version then, count).  A captured step advances its counter without the host, so from
+    # then on that one's count is not known; neither is it after someone else has written to it.
+    def _note(self, step, count):
+        known = self.__dict__.setdefault("_known", {})
+        known.pop(id(step), None)
+        if count is not None and not step.is_inference():
+            if len(known) > 2 * len(self.state):
+                used = {id(s["step"]) for s in self.state.values() if s}
+                for k in [k for k in known if k not in used]:
+                    del known[k]
+            known[id(step)] = (step, step._version, count)
+        return step
+
+    def _count(self, step):
+        held = self.__dict__.get("_known", {}).get(id(step))
+        return held[2] if held is not None and held[0] is step and held[1] == step._version else None
+
+    def _one_counter(self, ps, states, users):
+        """The counter of a list that steps now.  The list alone advances it: parameters that had it too but step in another list, or
+        not at all this time, keep the old count in the old one."""
+        here = {}
+        for state in states:
+            here[id(state["step"])] = here.get(id(state["step"]), 0) + 1
+        for state in states:
+            if users[id(state["step"])] == here[id(state["step"])]:
+                step = state["step"]
+                break
+        else:
+            _not_captured(ps[0], "a step of some of the parameters that have stepped together: their count would begin anew with every replay")
+            step = self._note(states[0]["step"].clone(), self._count(states[0]["step"]))
+        if len(here) > 1 or id(step) not in here:
+            for state in states:
+                state["step"] = step
+        return step
 
     def _check_checkpoint(self, state_dict):
         saved = state_dict["param_groups"]
@@ -163,7 +203,9 @@ class AdamW(torch.optim.Optimizer):
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             counters = {}
             for i, p in zip(saved["params"], group["params"]):
-                if i in state_dict["state"]:
+                if state_dict["state"].get(i):
                     state = {k: v.to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
-                    state["step"] = counters.setdefault((int(state["step"]), p.device), state["step"])
+                    count = int(state["step"])
+                    state["step"] = counters.setdefault((count, p.device), state["step"])
+                    self._note(state["step"], count)
                     self.state[p] = state
