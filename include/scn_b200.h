@@ -697,9 +697,9 @@ SCN_API int scn_grouped_product_quantized(const void *q, int64_t q_stride, const
                                           const float *weight_scale, const void *bias, int bias_type, const void *offsets,
                                           int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out, void *out, int out_type,
                                           void *stream);
-/* Every wait inside the grouped products is bounded; one that ran out leaves a flag.  Waits for `stream`, reads and clears the
- * current device's flag: SCN_ERR_CUDA if it was set.  scn_test_drop_barrier_arrival reaches the next
- * scn_grouped_product_forward too. */
+/* Every wait inside the grouped products is bounded; one that ran out leaves a flag of its device.  The next grouped product on that
+ * device that sees it clears it and returns SCN_ERR_CUDA without doing its own work; so does this call for the current device, after
+ * waiting for `stream`.  scn_test_drop_barrier_arrival reaches the next scn_grouped_product_forward too. */
 SCN_API int scn_rows_poll_errors(void *stream);
 
 #ifdef __cplusplus

@@ -34,11 +34,13 @@
 //   small groups  rows behind a group's last are not copied (boxes of 32 rows): their accumulator rows hold anything and are
 //               not stored.
 //
-// Every wait is bounded; what gave up is reported by scn_rows_poll_errors.
+// Every wait is bounded; what gave up is reported by the next call on the device, or by scn_rows_poll_errors.
 #include <cuda.h>
+#include <string.h>
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "rows.cuh"
 #include "tc_ptx.cuh"
@@ -55,8 +57,6 @@ constexpr int kMostGroups = 1024;
 constexpr int kDrain = 4;                    // steps (of four instructions a product) between two hand-overs
 constexpr int kLong = 128, kLongDrain = 64;  // long sums of 16- and 8-bit values: from how many steps on, and between two hand-overs
 constexpr int kMostStages = 8;
-
-__device__ int g_flag;  // set by a kernel that gave up
 
 struct GroupParams {
   const void *offsets;
@@ -81,6 +81,7 @@ struct GroupParams {
   int bias_type;
   const float *row_scale, *col_scale;
   int drop;                // test: leave out the first arrival
+  int *flag;               // pinned host memory: set by a kernel that gave up
 };
 
 struct Shared {
@@ -101,6 +102,11 @@ struct Unit {
   int group, row, rows, n0, m0;  // row: first row; rows: of the tile (rows) or of the sum (weights)
   int part;                      // weights: the partial sum that this unit makes, -1: the gradient itself
 };
+
+__device__ __forceinline__ void gave_up(const GroupParams &P) {
+  *(volatile int *)P.flag = 1;
+  __threadfence_system();
+}
 
 __device__ __forceinline__ int offset_at(const GroupParams &P, int g) {
   const long long v = P.off64 ? __ldg((const long long *)P.offsets + g) : (long long)__ldg((const int *)P.offsets + g);
@@ -596,7 +602,7 @@ k_group_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   tc_fence_after();
   if (S.abort) {  // what is under way into this block's memory lands before the block ends
     if (tid == 0) {
-      atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+      gave_up(P);
       for (int s = 0; s < kStages; ++s)
         if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
     }
@@ -905,7 +911,7 @@ k_group_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   tc_fence_after();
   if (S.abort) {  // own copies land before the block ends; those of full steps are counted by the leader
     if (tid == 0) {
-      atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+      gave_up(P);
       if (rank == 0)
         for (int s = 0; s < kStages; ++s)
           if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
@@ -1300,7 +1306,7 @@ k_group_split(const __grid_constant__ CUtensorMap map_b, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   if (S.abort && tid == 0) {  // the weights' copies land before the block ends
-    atomicOr(&g_flag, (int)FLAG_TC_TIMEOUT);
+    gave_up(P);
     // (a stage's barrier also counts the rows, which may not come any more: a bounded wait is long enough for a copy to land)
     for (int s = 0; s < kStages; ++s)
       if (S.issued > s) mbar_wait(&S.full[s], ((S.issued - 1 - s) / kStages) & 1);
@@ -1431,6 +1437,34 @@ int encoder(EncodeTiled *out) {  // looked up through the runtime: the library l
     SCN_REQUIRE(fn && found == cudaDriverEntryPointSuccess, SCN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     known.store(*out = (EncodeTiled)fn);
   }
+  return SCN_OK;
+}
+
+// Where kernels of the current device say that they gave up: a word of pinned memory, so that the next call sees it without waiting.
+int flag_of(int **word) {
+  static std::mutex mu;
+  static int *words = nullptr;
+  int dev = 0;
+  SCN_CUDA_CHECK(cudaGetDevice(&dev));
+  SCN_REQUIRE(dev >= 0 && dev < 64, SCN_ERR_UNSUPPORTED, "device index %d unsupported", dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (!words) {  // (allowed while a stream of this thread is captured: nothing of it becomes part of the graph)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SCN_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    void *p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, 64 * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    SCN_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    SCN_CUDA_CHECK(e);
+    memset(p, 0, 64 * sizeof(int));
+    words = (int *)p;
+  }
+  *word = words + dev;
+  return SCN_OK;
+}
+// An error if a call before this one gave up, once
+int look_at_flag(int *word) {
+  SCN_REQUIRE(!__atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL), SCN_ERR_CUDA,
+              "a wait inside an earlier grouped product ran out: its results are incomplete");
   return SCN_OK;
 }
 
@@ -1577,6 +1611,7 @@ struct Groups {
   int off64;
   long long n_rows;
   int groups;
+  int *flag;
 };
 
 // y = x W: `b_rows`: the weights' n lie next to each other ([k][n]), else their k ([n][k])
@@ -1589,7 +1624,7 @@ int rows_product(const Groups &G, const Operand &x, const Operand &w, bool b_row
   const bool pair = !fine && paired(pair_tiles, G.groups, n);
   const int tn = pair ? kPairN : tile_columns(row_tiles, n, fine ? 128 : 256);
   GroupParams P{};
-  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows, P.flag = G.flag;
   P.tile = pair ? 2 * kTileM : kTileM;
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(type, false, b_rows, P.tile);
@@ -1641,7 +1676,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   const long long m_tiles = ceil_div(m, pair ? 2 * kTileM : kTileM);
   const int tn = pair ? kPairN : tile_columns(m_tiles * std::max<long long>(G.groups, G.n_rows / 512), n, parts > 1 ? 128 : 256);
   GroupParams P{};
-  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows, P.flag = G.flag;
   P.tile = pair ? 2 * kTileM : kTileM;
   P.m = P.m_rows = m, P.n = n, P.m_tiles = (int)m_tiles, P.n_tiles = (int)ceil_div(n, tn);
   P.chunk = chunk_of(G.n_rows, (long long)P.m_tiles * P.n_tiles);
@@ -1703,7 +1738,7 @@ int rows_product_split(const Groups &G, const void *x, long long stride, const O
   const long long row_tiles = G.n_rows / kTileM + std::min<long long>(G.groups + 2, G.n_rows);
   const int tn = tile_columns(row_tiles, n, 128);
   GroupParams P{};
-  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows, P.flag = G.flag;
   P.tile = kTileM;
   P.k = k, P.n = n, P.n_tiles = (int)ceil_div(n, tn);
   P.idesc = idesc_of(SCN_TYPE_BFLOAT16, false, b_rows, kTileM);
@@ -1727,7 +1762,7 @@ int weights_product_split(const Groups &G, const void *x, long long x_stride, co
                           void *d_bias, bool *bias_done, Scratch &scratch, cudaStream_t stream) {
   const int tn = n <= 64 ? 64 : 128;
   GroupParams P{};
-  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows, P.flag = G.flag;
   P.tile = kTileM;
   *bias_done = d_bias && m % kTileM != 0;
   P.m = m, P.m_rows = m + *bias_done, P.n = n, P.m_tiles = (int)ceil_div(m, kTileM), P.n_tiles = (int)ceil_div(n, tn);
@@ -1748,7 +1783,7 @@ int weights_product_split(const Groups &G, const void *x, long long x_stride, co
 
 int bias_sums(const Groups &G, const void *dy, long long stride, int type, int n, void *out, int out_type, Scratch &scratch, cudaStream_t stream) {
   GroupParams P{};
-  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows;
+  P.offsets = G.offsets, P.off64 = G.off64, P.groups = G.groups, P.n_rows = (int)G.n_rows, P.flag = G.flag;
   P.m = P.m_rows = 1, P.n = n, P.m_tiles = P.n_tiles = 1;
   P.chunk = chunk_of(G.n_rows, std::max<long long>(1, ceil_div(n, 32) / 4));
   P.out = out, P.out_type = out_type;
@@ -1799,7 +1834,10 @@ int scn_grouped_product_forward(const void *x, int64_t x_stride, int type, const
   SCN_TRY(check_sizes(offsets, n_rows, n_groups, n_in, n_out));
   if (n_rows == 0) return SCN_OK;
   SCN_REQUIRE(x && weight && out, SCN_ERR_BAD_ARG, "grouped_product: null argument");
-  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  int *flag = nullptr;
+  SCN_TRY(flag_of(&flag));
+  SCN_TRY(look_at_flag(flag));
+  const Groups G{offsets, offsets_64, n_rows, n_groups, flag};
   const int parts = parts_of(type, precision), held = type == SCN_TYPE_FLOAT32 ? SCN_TYPE_BFLOAT16 : type;
   const int drop = g_drop_arrival;
   g_drop_arrival = 0;
@@ -1826,7 +1864,10 @@ int scn_grouped_product_backward(const void *x, int64_t x_stride, int type, cons
     return SCN_OK;
   }
   SCN_REQUIRE(d_out && (!d_x || weight) && (!d_weight || x), SCN_ERR_BAD_ARG, "grouped_product: null argument");
-  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  int *flag = nullptr;
+  SCN_TRY(flag_of(&flag));
+  SCN_TRY(look_at_flag(flag));
+  const Groups G{offsets, offsets_64, n_rows, n_groups, flag};
   const int held = type == SCN_TYPE_FLOAT32 ? SCN_TYPE_BFLOAT16 : type;
   // the input's gradient at the precision asked for, the weights' always as fp32
   const int dx_parts = parts_of(type, precision), dw_parts = parts_of(type, SCN_PRECISION_FP32);
@@ -1861,7 +1902,10 @@ int scn_grouped_product_quantized(const void *q, int64_t q_stride, const float *
   SCN_TRY(check_sizes(offsets, n_rows, n_groups, n_in, n_out));
   if (n_rows == 0) return SCN_OK;
   SCN_REQUIRE(q && scale && weight && weight_scale && out, SCN_ERR_BAD_ARG, "grouped_product: null argument");
-  const Groups G{offsets, offsets_64, n_rows, n_groups};
+  int *flag = nullptr;
+  SCN_TRY(flag_of(&flag));
+  SCN_TRY(look_at_flag(flag));
+  const Groups G{offsets, offsets_64, n_rows, n_groups, flag};
   Scratch scratch(stream);
   Operand a, b;
   SCN_TRY(operand(q, q_stride, n_in, n_rows, SCN_TYPE_E4M3, 1, scratch, stream, &a));
@@ -1872,14 +1916,11 @@ int scn_grouped_product_quantized(const void *q, int64_t q_stride, const float *
 
 int scn_rows_poll_errors(void *stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
-  int *at = nullptr, flag = 0;
-  SCN_CUDA_CHECK(cudaGetSymbolAddress((void **)&at, g_flag));
-  SCN_CUDA_CHECK(cudaMemcpyAsync(&flag, at, sizeof(int), cudaMemcpyDeviceToHost, stream));
+  int *flag = nullptr;
+  SCN_TRY(flag_of(&flag));
   note_host_wait();
   SCN_CUDA_CHECK(cudaStreamSynchronize(stream));
-  if (!flag) return SCN_OK;
-  SCN_CUDA_CHECK(cudaMemsetAsync(at, 0, sizeof(int), stream));
-  SCN_REQUIRE(false, SCN_ERR_CUDA, "a wait inside a grouped product ran out: its results are incomplete");
+  return look_at_flag(flag);
 }
 
 }  // extern "C"

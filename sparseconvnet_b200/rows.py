@@ -77,6 +77,7 @@ def grouped_product_quantized(q, scale, weight, weight_scale, offsets, bias=None
 
 
 def poll_errors():
-    """Waits for the current stream and raises if a wait inside a grouped product ran out since the last call (its results are
-    incomplete then).  The counterpart of ``Metadata.poll_errors``."""
+    """Waits for the current stream and raises if a wait inside a grouped product of the current device ran out (its results are
+    incomplete then).  A later grouped product raises this without waiting; what is behind the last one, or in a replayed graph,
+    shows here.  The counterpart of ``Metadata.poll_errors``."""
     SCN.check(SCN.lib.scn_rows_poll_errors(SCN._stream()))
