@@ -14,6 +14,7 @@
 // only, with more the warps of a row meet at one barrier per sum.  Blocks stay for the whole launch; a thread's weights are
 // read once, and the next row is asked for before the present one is summed.
 #include <algorithm>
+#include <atomic>
 
 #include "rows.cuh"
 
@@ -454,6 +455,21 @@ int add_blocks(const float *partial, long long blocks, int planes, float *out, c
   return SCN_OK;
 }
 
+// The shared memory that a block of `kernel` may have, for its weights' sums at most.  It belongs to the kernel, not to a call:
+// set once per device, so that two threads' calls of different widths do not take each other's away.
+template <auto kernel>
+int allow_shared() {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  SCN_CUDA_CHECK(cudaGetDevice(&dev));
+  SCN_REQUIRE(dev >= 0 && dev < 64, SCN_ERR_UNSUPPORTED, "device index %d unsupported", dev);
+  if (!configured[dev].load()) {
+    SCN_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(float) * kMostLanes * 4 * 8)));
+    configured[dev].store(true);
+  }
+  return SCN_OK;
+}
+
 template <typename T, int V, bool SAME>
 int launch_back(NormBackParams P, int chunks, float *d_weight, cudaStream_t stream) {
   const int threads = std::max(kThreads, P.lanes);
@@ -464,9 +480,7 @@ int launch_back(NormBackParams P, int chunks, float *d_weight, cudaStream_t stre
 #define SCN_NORM(CH)                                                                                           \
   case CH: {                                                                                                   \
     int most = 0;                                                                                              \
-    if (smem > 48 * 1024)                                                                                      \
-      SCN_CUDA_CHECK(cudaFuncSetAttribute(k_rms_norm_back<T, V, CH, SAME>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                          (int)smem));                                                         \
+    if (smem > 48 * 1024) SCN_TRY((allow_shared<k_rms_norm_back<T, V, CH, SAME>>()));                          \
     SCN_TRY((resident_blocks<k_rms_norm_back<T, V, CH, SAME>>(threads, 0, &most)));                                  \
     blocks = std::min<long long>(need, most);                                                                  \
     if (d_weight) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)blocks * P.planes));                 \

@@ -9,9 +9,11 @@ pytestmark = pytest.mark.gpu
 
 
 # one block to a tile, two, fp32 rows that the kernel splits, and long sums of one block and of two
-@pytest.mark.parametrize("rows,k,n,t", [(256, 4096, 256, torch.bfloat16), (20000, 4096, 512, torch.bfloat16), (200000, 256, 64, torch.float32),
-                                        (130, 16384, 200, torch.float16), (2600, 16384, 2304, torch.bfloat16)])
-@pytest.mark.parametrize("then", ["forward", "backward", "quantized"])
+SHAPES = [(256, 4096, 256, torch.bfloat16), (20000, 4096, 512, torch.bfloat16), (200000, 256, 64, torch.float32), (130, 16384, 200, torch.float16),
+          (2600, 16384, 2304, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("rows,k,n,t,then", [(*s, "forward") for s in SHAPES] + [(*SHAPES[0], then) for then in ("backward", "quantized")])
 def test_the_next_call_says_so(cuda, rows, k, n, t, then):
     """One arrival is left out: the call gives up in bounded time, and the next one on the device raises, once."""
     o = torch.tensor([0, rows], device="cuda")
