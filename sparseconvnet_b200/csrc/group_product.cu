@@ -1660,6 +1660,13 @@ int chunk_of(long long n_rows, long long tiles) {
   return (int)std::max<long long>(512, ceil_div(ceil_div(n_rows, wanted), 64) * 64);
 }
 
+// The most units that groups of several units can have together: such a group has more than `chunk` rows, so there are at most K of
+// them, and each rounds its rows / chunk up by less than one.
+long long most_parts(const Groups &G, long long chunk) {
+  const long long K = std::min<long long>(G.groups, G.n_rows / (chunk + 1));
+  return (G.n_rows + K * (chunk - 1)) / chunk;
+}
+
 int sum_parts(GroupParams P, cudaStream_t stream) {
   const long long items = ceil_div((long long)P.m_rows * P.n, 32) * P.groups;
   SCN_LAUNCH(k_group_sum, (unsigned)std::min<long long>(items, 8 * kSms), 256, 0, stream, P);
@@ -1684,8 +1691,7 @@ int weights_product(const Groups &G, const Operand &x, const Operand &dy, int pa
   const int out_size = out_type == SCN_TYPE_FLOAT32 ? 4 : 2;
   P.out = out, P.out_type = out_type, P.aligned = aligned_to((uintptr_t)out, n, out_size), P.part_aligned = aligned_to(0, n, 4);
   const bool split = G.n_rows > P.chunk;
-  // (a group of several units has more than P.chunk rows: at most n_rows / chunk of them, with one unit more each than that)
-  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * m * n));
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)most_parts(G, P.chunk) * m * n));
   CUtensorMap a, b;
   SCN_TRY(make_map(&a, x, type, m, G.n_rows, parts, 1, 64, kStageRows));
   SCN_TRY(make_map(&b, dy, type, n, G.n_rows, parts, 1, 64, kStageRows));
@@ -1755,8 +1761,9 @@ int rows_product_split(const Groups &G, const void *x, long long stride, const O
 #undef SCN_TN
 }
 
-// weights_product of fp32 rows, split in the kernel, with the bias sums where they fit (*bias_done).  Its units are short, so
-// the partial sums have to be small beside the rows: 256 rows of m + n values against m n sums.
+// weights_product of fp32 rows, split in the kernel, with the bias sums where they fit (*bias_done).  Its units are short, and 256
+// rows of m + n values bring m n partial sums: at most a third as many, for 128 x 256.  (Parts in memory would be one and a half
+// times the rows.)
 bool splits_weights(int type, int m, int n) { return type == SCN_TYPE_FLOAT32 && m <= 128 && n <= 256; }
 int weights_product_split(const Groups &G, const void *x, long long x_stride, const void *dy, long long dy_stride, int m, int n, void *out,
                           void *d_bias, bool *bias_done, Scratch &scratch, cudaStream_t stream) {
@@ -1774,7 +1781,7 @@ int weights_product_split(const Groups &G, const void *x, long long x_stride, co
   P.a = (const float *)x, P.a_stride = x_stride, P.a_quads = quads_of(x, x_stride, m);
   P.b = (const float *)dy, P.b_stride = dy_stride, P.b_quads = quads_of(dy, dy_stride, n);
   const bool split = G.n_rows > P.chunk;
-  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * P.m_rows * n));
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)most_parts(G, P.chunk) * P.m_rows * n));
   const long long most = (ceil_div(G.n_rows, P.chunk) + G.groups) * P.m_tiles * P.n_tiles;
   const CUtensorMap none{};
   SCN_TRY((tn == 64 ? launch_split<3, 64, true, true>(none, P, most, stream) : launch_split<3, 128, true, true>(none, P, most, stream)));
@@ -1788,7 +1795,7 @@ int bias_sums(const Groups &G, const void *dy, long long stride, int type, int n
   P.chunk = chunk_of(G.n_rows, std::max<long long>(1, ceil_div(n, 32) / 4));
   P.out = out, P.out_type = out_type;
   const bool split = G.n_rows > P.chunk;
-  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)(2 * (G.n_rows / P.chunk)) * n));
+  if (split) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)most_parts(G, P.chunk) * n));
   const long long units = ceil_div(G.n_rows, P.chunk) + G.groups;
   const dim3 grid((unsigned)ceil_div(n, 32), (unsigned)std::min<long long>(units, 1024));
   if (type == SCN_TYPE_FLOAT32)
