@@ -681,7 +681,7 @@ SCN_API int scn_adamw_step(const scn_adamw_tensor *tensors, int64_t n_tensors, i
  * and zeros for rows of no group.  offsets [n_groups + 1]: DEVICE int64 (offsets_64 != 0) or int32, not decreasing, within
  * [0, n_rows]; they are clamped to that, and rows of groups that overlap all the same are undefined.  At most 1024 groups.
  * 16-bit operands are multiplied as they are, float32 ones according to `precision` (an scn_precision): FP32 as three bf16
- * parts and six products, TF32 and TF32X3 as two parts and three, BF16 as one.  Sums are float32.  In float32 an infinity
+ * parts and six products (all bits of values from 2^-110 on, smaller ones to within 2^-134), TF32 and TF32X3 as two parts and three, BF16 as one.  Sums are float32.  In float32 an infinity
  * may become NaN (FP32, TF32X3, TF32). */
 SCN_API int scn_grouped_product_forward(const void *x, int64_t x_stride, int type, const void *weight, const void *bias, int bias_type,
                                         const void *offsets, int offsets_64, int64_t n_rows, int n_groups, int n_in, int n_out,

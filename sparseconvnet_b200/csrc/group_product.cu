@@ -13,8 +13,8 @@
 // k_group_pair takes wide layers and large groups, k_group_split fp32 rows of few planes.
 //
 //   arithmetic  16-bit and 8-bit values as they are, fp32 sums.  fp32 values as bf16 parts (k_group_parts): x = h + m + l
-//               holds all 24 bits, and the products h h, h m, m h, h l, l h, m m leave out 2^-24 of a product; two parts and
-//               h h, h m, m h leave out 2^-17.  The tensor core cuts its running sum off at every instruction, half a unit
+//               holds all 24 bits of values from 2^-110 on (below that l ends at bf16's smallest number, 2^-133), and the
+//               products h h, h m, m h, h l, l h, m m leave out 2^-24 of a product; two parts and h h, h m, m h leave out 2^-17.  The tensor core cuts its running sum off at every instruction, half a unit
 //               of 2^-24 of it on average, so for fp32 results of fp32 and 16-bit values a sum is handed over to the registers
 //               of the epilogue warps every kDrain steps, and the products with an m or l have an accumulator of their own
 //               (they are 2^-8 as large).  Results of fewer bits, and all results of 8-bit values, take a sum of up to kLong

@@ -50,7 +50,8 @@ def grouped_product(x, weight, offsets, bias=None, out_dtype=None):
     them.  Rows of no group (before the first, behind the last) are zeros and have no gradient.
     bfloat16 and float16 are multiplied as they are; float32 by ``set_precision``: 'fp32' with all bits, 'tf32x3' and 'tf32'
     to 2^-17 of a product, 'bf16' rounded to bfloat16 (the input's gradient by ``set_backward_precision``, the weights'
-    with all bits).  Sums are float32, results ``out_dtype`` (None: the type of x).  A float32 row with an infinity may
+    with all bits).  In 'fp32' values below 2^-110 (8e-34) are held to within 2^-134.  Sums are float32, results ``out_dtype``
+    (None: the type of x); the gradient of float32 results of 16-bit operands is rounded to the operands' type first.  A float32 row with an infinity may
     give NaN.  Differentiable (once) in x, weight and bias."""
     return SCN._binding.grouped_product(x, weight, offsets, bias, _type_code(out_dtype, "out_dtype"), SCN._precision,
                                         SCN._backward_precision)
