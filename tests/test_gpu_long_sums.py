@@ -92,3 +92,26 @@ def test_lengths_around_a_hand_over(cuda, t):
         again, = torch.autograd.grad(scn.grouped_product(x, w, o), [w], dy)
         assert torch.equal(dw, again)
         scn.poll_errors()
+
+
+@pytest.mark.parametrize("t", [torch.float32, *HALF])
+@pytest.mark.parametrize("rows,nout", [(130, 203), (2600, 2303), (2600, 2320), (19000, 264)])
+def test_every_way_out(cuda, rows, nout, t):
+    """Results of all types, in rows of any alignment, with a bias: 16-bit operands (but for float32 results, whose sums are short), and 8-bit
+    ones"""
+    k = 20000
+    o = torch.tensor([3, 80, rows - 1], device="cuda")
+    parts = ((slice(3, 80), 0), (slice(80, rows - 1), 1))
+    half = t if t != torch.float32 else torch.float16
+    x, w, b = positive(rows, k, t=half, seed=1), positive(2, k, nout, t=half, seed=2, most=0.25), positive(2, nout, t=half, seed=3, most=900.0)
+    y = scn.grouped_product(x, w, o, b, out_dtype=t)
+    q, v = positive(rows, k, t=torch.float8_e4m3fn, seed=4, most=400.0), positive(2, nout, k, t=torch.float8_e4m3fn, seed=5, most=400.0)
+    scale, ws = positive(rows, t=torch.float32, seed=6) * 1e-5 + 1e-5, positive(2, nout, t=torch.float32, seed=7) * 1e-2 + 1e-2
+    z = scn.grouped_product_quantized(q, scale, v, ws, o, b, out_dtype=t)
+    for r, g in parts:
+        for c in (slice(0, 70), slice(nout - 70, nout)):
+            check(y[r, c], x[r].double() @ w[g, :, c].double() + b[g, c].double(), k / 4096 + 1, t, others=2 * E)
+            check(z[r, c], q[r].double() @ v[g, c].double().T * scale[r].double()[:, None] * ws[g, c].double() + b[g, c].double(), k / 8192 + 1, t, others=4 * E)
+    outside = torch.tensor([0, 1, 2, rows - 1], device="cuda")
+    assert bool((y[outside] == 0).all()) and bool((z[outside] == 0).all())
+    scn.poll_errors()
