@@ -115,3 +115,47 @@ def test_every_way_out(cuda, rows, nout, t):
     outside = torch.tensor([0, 1, 2, rows - 1], device="cuda")
     assert bool((y[outside] == 0).all()) and bool((z[outside] == 0).all())
     scn.poll_errors()
+
+
+@pytest.mark.parametrize("t", HALF)
+def test_many_groups_of_many_planes(cuda, t):
+    """Tiles of one block and 256 columns: groups too small for two blocks to a tile, 300 and 100 columns for narrower ones"""
+    k, groups = 9000, 90
+    o = torch.arange(groups + 1, device="cuda") * 31
+    rows = int(o[-1])
+    x = positive(rows, k, t=t, seed=1)
+    for nout in (1000, 300, 100):
+        w = positive(groups, k, nout, t=t, seed=2, most=0.25)
+        y = scn.grouped_product(x, w, o)
+        v, z = w.transpose(1, 2).contiguous(), torch.zeros(rows, nout, device="cuda", dtype=t, requires_grad=True)
+        (dz,) = torch.autograd.grad(scn.grouped_product(z, v, o), [z], x)
+        for g in (0, 1, 44, 89):
+            r = slice(31 * g, 31 * g + 31)
+            want = x[r].double() @ w[g].double()
+            check(y[r], want, k / 4096 + 1, t)
+            check(dz[r], want, k / 4096 + 1, t)
+    q, v = positive(rows, 2 * k, t=torch.float8_e4m3fn, seed=4, most=400.0), positive(groups, 1000, 2 * k, t=torch.float8_e4m3fn, seed=5, most=400.0)
+    scale, ws = positive(rows, t=torch.float32, seed=6) * 1e-5 + 1e-5, positive(groups, 1000, t=torch.float32, seed=7) * 1e-2 + 1e-2
+    y = scn.grouped_product_quantized(q, scale, v, ws, o, out_dtype=t)
+    for g in (0, 44, 89):
+        r = slice(31 * g, 31 * g + 31)
+        check(y[r], q[r].double() @ v[g].double().T * scale[r].double()[:, None] * ws[g].double(), 2 * k / 8192 + 1, t, others=4 * E)
+
+
+@pytest.mark.parametrize("nin,nout", [(64, 64), (100, 128), (128, 72)])
+def test_millions_of_rows(cuda, nin, nout):
+    """A result of a tile or two: units of a 300th of the rows, each of them long"""
+    rows, t = 3000017, torch.bfloat16
+    o = torch.tensor([0, 9001, rows - 11, rows], device="cuda")
+    x, dy = positive(rows, nin, t=t, seed=1), positive(rows, nout, t=t, seed=2, most=0.25)
+    w, b = torch.zeros(3, nin, nout, device="cuda", dtype=t, requires_grad=True), torch.zeros(3, nout, device="cuda", dtype=t, requires_grad=True)
+    dw, db = torch.autograd.grad(scn.grouped_product(x, w, o, b), [w, b], dy)
+    for g in range(3):
+        r = slice(int(o[g]), int(o[g + 1]))
+        want, sums = torch.zeros(nin, nout, device="cuda", dtype=torch.float64), torch.zeros(nout, device="cuda", dtype=torch.float64)
+        for s in range(r.start, r.stop, 500000):
+            e = min(r.stop, s + 500000)
+            want += x[s:e].double().T @ dy[s:e].double()
+            sums += dy[s:e].double().sum(0)
+        check(dw[g], want, 3, t, others=300 * E)  # (the partial sums of 300 units, one after the other)
+        check(db[g], sums, 0, t, others=(10200 / 64 + 300 + 20) * E)
