@@ -279,7 +279,7 @@ __device__ __forceinline__ float value_at(const void *p, int type, long long i) 
 }
 
 // 32 results of a row, `left` of them in the row, in rows that begin at multiples of `aligned` bytes: 8, 16 or 32.  32: whole
-// sectors (pieces of 16 bytes reach L2 as two writes of half a sector: group_wide_8bit took 70 us more).
+// sectors (pieces of 16 bytes reach L2 as two writes of half a sector: group_wide_8bit took 70 us more).  Inlined only (rows.cuh).
 template <int WORDS>
 __device__ __forceinline__ void store_words32(void *to, int aligned, int left, const unsigned (&w)[WORDS]) {
   constexpr int kPer = 32 / WORDS;  // values of a word

@@ -52,7 +52,8 @@ __device__ __forceinline__ void pack8(const float (&v)[8], unsigned (&w)[8], flo
 }
 
 // N words of a stream that is read or written once, past L1.  8 words are one access of 32 bytes, a whole sector: as two of
-// 16 bytes the neighbouring lanes' accesses lie 32 bytes apart, and every sector is asked for twice.
+// 16 bytes the neighbouring lanes' accesses lie 32 bytes apart, and every sector is asked for twice.  The 32-byte store belongs into
+// code that is inlined: in a __noinline__ function nvcc 12.9 stored other registers in place of all but the first word.
 __device__ __forceinline__ void load_words(const void *p, unsigned (&w)[4]) {
   asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
