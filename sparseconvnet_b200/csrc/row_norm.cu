@@ -455,7 +455,8 @@ int add_blocks(const float *partial, long long blocks, int planes, float *out, c
   return SCN_OK;
 }
 
-// The shared memory that a block of `kernel` may have, for its weights' sums at most.  It belongs to the kernel, not to a call:
+// The shared memory that a block of `kernel` may have, for its weights' sums at most.  (Without it a block has 48 KB, what the
+// kernel declares by itself included.)  It belongs to the kernel, not to a call:
 // set once per device, so that two threads' calls of different widths do not take each other's away.
 template <auto kernel>
 int allow_shared() {
@@ -480,7 +481,7 @@ int launch_back(NormBackParams P, int chunks, float *d_weight, cudaStream_t stre
 #define SCN_NORM(CH)                                                                                           \
   case CH: {                                                                                                   \
     int most = 0;                                                                                              \
-    if (smem > 48 * 1024) SCN_TRY((allow_shared<k_rms_norm_back<T, V, CH, SAME>>()));                          \
+    if (smem > 32 * 1024) SCN_TRY((allow_shared<k_rms_norm_back<T, V, CH, SAME>>()));                          \
     SCN_TRY((resident_blocks<k_rms_norm_back<T, V, CH, SAME>>(threads, 0, &most)));                                  \
     blocks = std::min<long long>(need, most);                                                                  \
     if (d_weight) SCN_TRY(scratch.get(&P.partial, sizeof(float) * (size_t)blocks * P.planes));                 \
